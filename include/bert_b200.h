@@ -76,6 +76,18 @@ BERT_B200_API int32_t bert_b200_skip_layer_norm(void* stream, int32_t type_id, i
     void const* input, void const* skip, void const* beta, void const* gamma, void* output, void const* bias);
 
 /*
+ * The same row quantised to INT8 with a scale of its own (what bert_b200_fc_rowwise multiplies):
+ *   y = gamma * (x - mean(x)) * rsqrt(var(x) + eps) + beta as above (skip may be NULL: plain LayerNorm; output may be NULL),
+ *   row_scales[r] = max|y| / 127, out_i8 = rni(127 y / max|y|), from the FP32 y before it is rounded to the output's type.
+ * A row of zeros has scale 0, a row with a NaN or an infinity scale NaN and out_i8 = 0. `output` has the bits that
+ * bert_b200_skip_layer_norm gives for the same eps (its FP16 form has eps 0). type_id 0 or 1. output may be input or skip.
+ * ref: none (one calibrated step per tensor: bert_b200_skip_layer_norm_dqq)
+ */
+BERT_B200_API int32_t bert_b200_skip_layer_norm_quantize(void* stream, int32_t type_id, int32_t ld, int64_t n,
+    void const* input, void const* skip, void const* beta, void const* gamma, void* output, int8_t* out_i8,
+    float* row_scales, void const* bias, float eps);
+
+/*
  * INT8 in / INT8 out, linear layout: x = dq_scale_in*input + dq_scale_skip*skip (+ bias),
  * out = sat8(rni(LN(x) * q_scale)). beta/gamma/bias are FP16. ld % 16 == 0.
  * ref: plugin/skipLayerNormPlugin/skipLayerNormKernel.cu:219-250 (computeSkipLayerNormDQQ<hasBias>)
@@ -233,6 +245,44 @@ typedef struct bert_b200_fc_params
 
 BERT_B200_API int32_t bert_b200_fc(bert_b200_fc_params const* params, void* stream);
 
+/*
+ * Quantises each row with a scale of its own: row_scales[r] = max|x[r]| / 127, output[r] = x[r] * 127 / max|x[r]| rounded to the nearest
+ * whole number (halves to even; the rounding is that of the exact quotient). type_id 0 or 1; strides in elements, at least `width`.
+ * A row of zeros has scale 0 and q 0; a row with a NaN or an infinity has scale NaN and q 0, so that what is multiplied with it is NaN.
+ * Any width, strides and alignment; 16-byte aligned rows of up to 8192 halves or 4096 floats (and output rows aligned to 8 or 4 bytes) take the
+ * kernel that reads them once. Weights [n][k] become per-channel INT8 the same way, once.
+ * ref: none (one step per tensor there: tools/pytorch-quantization/pytorch_quantization/tensor_quant.py:511-556)
+ */
+BERT_B200_API int32_t bert_b200_quantize_rows(void* stream, int32_t type_id, int64_t rows, int32_t width, void const* input,
+    int64_t input_stride, int8_t* output, int64_t output_stride, float* row_scales);
+
+/*
+ * C[m,n] = act( (sum_k A[m,k] * Wt[n,k]) * a_scales[m] * wt_scales[n] + bias[n] ): INT8 operands with a scale for each row of A (token) and
+ * each output channel, INT32 sums (exact; k <= 131071), C FP16 or FP32 (out_type_id 1 or 0), bias FP32 or NULL, act per `activation`.
+ * Any m, n and k; lda, ldw, ldc are row strides in elements, each a multiple of 16 bytes; A, Wt, C, wt_scales and bias 16-byte aligned.
+ * Only the m x n values of C are written. A row of C has the same bits whatever m. With FP16 results the GELU is the fitted form of
+ * bert_b200_fc (below FP16 resolution), with FP32 results erff. `status_word` as in bert_b200_fc.
+ * ref: none (plugin/fcPlugin/fcPlugin.cpp:551-610 has no INT8 scales)
+ */
+typedef struct bert_b200_fc_rowwise_params
+{
+    int32_t out_type_id;
+    int32_t activation;
+    int64_t m, n, k;
+    int8_t const* a;
+    int64_t lda;
+    float const* a_scales; /* [m] */
+    int8_t const* wt;
+    int64_t ldw;
+    float const* wt_scales; /* [n] */
+    void* c;
+    int64_t ldc;
+    float const* bias;
+    uint32_t* status_word;
+} bert_b200_fc_rowwise_params;
+
+BERT_B200_API int32_t bert_b200_fc_rowwise(bert_b200_fc_rowwise_params const* params, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Fused multi-head attention
  * ------------------------------------------------------------------------------------------ */
@@ -337,6 +387,39 @@ BERT_B200_API int32_t bert_b200_selftest_wait_expiry(void* stream, int64_t limit
  */
 BERT_B200_API int32_t bert_b200_probe_mma_rate(void* stream, int32_t type_id, int32_t k_blocks, uint32_t* status_word,
     float* tera_ops_host);
+
+/* ------------------------------------------------------------------------------------------
+ * Answers of a language-model head
+ * ------------------------------------------------------------------------------------------ */
+
+/*
+ * For each row of logits [rows][vocab] (type_id 0 or 1, row stride `logits_stride` in elements, any alignment), in one pass:
+ *   log_probs[rows][num_tokens]  log softmax(row)[token_ids[row][j]]
+ *   entropy[rows]                -sum p ln p (NULL: not wanted)
+ *   top_ids, top_log_probs [rows][top_k]  the most likely tokens, most likely first, of equal logits the lower id first; top_k <= 32
+ * all FP32 (ids int32). A logit of -infinity is a token of probability 0: its log probability is -infinity and it is no alternative;
+ * where fewer than top_k tokens are left the rest is -1 / -infinity. A row of nothing but -infinity: log probabilities -infinity, entropy
+ * 0, no alternatives. A row with a NaN or +infinity: NaN, ids -1. A token id outside [0, vocab) has probability 0 (-infinity).
+ * num_tokens and top_k may be 0; vocab is at most 2^24. Log probabilities keep their digits near 0 (a row that is sure of a token).
+ * ref: none (the reference's plugins end at the encoder's output)
+ */
+typedef struct bert_b200_log_probs_params
+{
+    int32_t type_id;
+    int64_t rows;
+    int32_t vocab;
+    void const* logits;
+    int64_t logits_stride;
+    int32_t num_tokens;
+    int32_t const* token_ids;
+    int32_t top_k;
+    float* log_probs;
+    float* entropy;
+    int32_t* top_ids;
+    float* top_log_probs;
+} bert_b200_log_probs_params;
+
+BERT_B200_API int32_t bert_b200_token_log_probs(bert_b200_log_probs_params const* params, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Whole-encoder driver (host layer loop over the kernels above)

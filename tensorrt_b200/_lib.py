@@ -43,6 +43,18 @@ class AttentionBnsdParams(C.Structure):
                 ("scale_bmm2", f32), ("status_word", vp)]
 
 
+class FcRowwiseParams(C.Structure):
+    _fields_ = [("out_type_id", i32), ("activation", i32), ("m", i64), ("n", i64), ("k", i64), ("a", vp), ("lda", i64),
+                ("a_scales", vp), ("wt", vp), ("ldw", i64), ("wt_scales", vp), ("c", vp), ("ldc", i64), ("bias", vp),
+                ("status_word", vp)]
+
+
+class LogProbsParams(C.Structure):
+    _fields_ = [("type_id", i32), ("rows", i64), ("vocab", i32), ("logits", vp), ("logits_stride", i64),
+                ("num_tokens", i32), ("token_ids", vp), ("top_k", i32), ("log_probs", vp), ("entropy", vp),
+                ("top_ids", vp), ("top_log_probs", vp)]
+
+
 class LayerWeights(C.Structure):
     _fields_ = [("wt_qkv", vp), ("b_qkv", vp), ("wt_out", vp), ("b_out", vp), ("ln1_gamma", vp), ("ln1_beta", vp),
                 ("wt_ffn1", vp), ("b_ffn1", vp), ("wt_ffn2", vp), ("b_ffn2", vp), ("ln2_gamma", vp), ("ln2_beta", vp),
@@ -63,6 +75,7 @@ SIGNATURES = {
     "bert_b200_last_error": (C.c_char_p, []),
     "bert_b200_read_status_word": (i32, [vp, vp, C.POINTER(u32)]),
     "bert_b200_skip_layer_norm": (i32, [vp, i32, i32, i64, vp, vp, vp, vp, vp, vp]),
+    "bert_b200_skip_layer_norm_quantize": (i32, [vp, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp, vp, f32]),
     "bert_b200_skip_layer_norm_dqq": (i32, [vp, i32, i64, vp, vp, vp, vp, vp, vp, f32, f32, f32]),
     "bert_b200_skip_layer_norm_interleaved_hface": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, f32, f32, f32]),
     "bert_b200_skip_layer_norm_interleaved_mtron": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, vp, f32, f32, f32, f32]),
@@ -74,6 +87,9 @@ SIGNATURES = {
     "bert_b200_packed_mask_to_lengths": (i32, [vp, i32, i32, u32, u32, u32, vp, vp]),
     "bert_b200_lengths_to_cu_seqlens": (i32, [vp, i32, vp, vp]),
     "bert_b200_fc": (i32, [C.POINTER(FcParams), vp]),
+    "bert_b200_quantize_rows": (i32, [vp, i32, i64, i32, vp, i64, vp, i64, vp]),
+    "bert_b200_fc_rowwise": (i32, [C.POINTER(FcRowwiseParams), vp]),
+    "bert_b200_token_log_probs": (i32, [C.POINTER(LogProbsParams), vp]),
     "bert_b200_attention_bnsd": (i32, [C.POINTER(AttentionBnsdParams), vp]),
     "bert_b200_mha_workspace_size": (i64, [C.POINTER(MhaParams)]),
     "bert_b200_mha": (i32, [C.POINTER(MhaParams), vp]),

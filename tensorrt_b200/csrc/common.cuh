@@ -257,6 +257,22 @@ __device__ __forceinline__ float warpMax(float v)
     return v;
 }
 
+// NaN if either is NaN.
+__device__ __forceinline__ float maxNan(float a, float b)
+{
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+    return v;
+}
+
+__device__ __forceinline__ float warpMaxNan(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        v = maxNan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
 // 128-bit global load through the read-only path, no L1 allocation (streamed once).
 __device__ __forceinline__ uint4 ldgStream(void const* p)
 {

@@ -1,0 +1,232 @@
+// Rows of FP16 / FP32 activations to INT8, each with a scale of its own (see row_quant.cuh for the arithmetic): what the row-wise INT8
+// layers multiply. No counterpart in the reference, whose INT8 plugins take one calibrated step per tensor.
+#include "row_quant.cuh"
+
+namespace b200
+{
+namespace
+{
+
+constexpr int kThreads = 256;
+
+// The row's maximum over WPR warps; `slots`: this row's scratch, two lines used alternately (one barrier per call is enough, see rowSum
+// in skip_ln.cu).
+template <int WPR>
+__device__ __forceinline__ float rowMax(float v, float (*slots)[WPR], int rowInCta, int wInRow, int lane, int& turn)
+{
+    v = warpMaxNan(v);
+    if (WPR == 1)
+        return v;
+    float* const slot = slots[turn];
+    turn ^= 1;
+    if (lane == 0)
+        slot[wInRow] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + rowInCta), "n"(WPR * 32) : "memory");
+    float t = slot[0];
+#pragma unroll
+    for (int w = 1; w < WPR; ++w)
+        t = maxNan(t, slot[w]);
+    return t;
+}
+
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<__half>
+{
+    static constexpr int kElems = 8;
+    static __device__ __forceinline__ float absMax(uint4 const& v)
+    {
+        __half2 const* h = reinterpret_cast<__half2 const*>(&v);
+        __half2 const m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+        return maxNan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ void unpack(uint4 const& v, float (&f)[8])
+    {
+        unpackHalf8(v, f);
+    }
+    // `n` of the eight values, zeros behind them
+    static __device__ __forceinline__ uint4 loadPart(__half const* p, int n)
+    {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n)
+                w[j / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<unsigned short const*>(p) + j)) << (16 * (j & 1));
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <>
+struct Chunk<float>
+{
+    static constexpr int kElems = 4;
+    static __device__ __forceinline__ float absMax(uint4 const& v)
+    {
+        return maxNan(maxNan(fabsf(__uint_as_float(v.x)), fabsf(__uint_as_float(v.y))), maxNan(fabsf(__uint_as_float(v.z)), fabsf(__uint_as_float(v.w))));
+    }
+    static __device__ __forceinline__ void unpack(uint4 const& v, float (&f)[4])
+    {
+        f[0] = __uint_as_float(v.x);
+        f[1] = __uint_as_float(v.y);
+        f[2] = __uint_as_float(v.z);
+        f[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 loadPart(float const* p, int n)
+    {
+        return make_uint4(n > 0 ? __float_as_uint(__ldg(p)) : 0u, n > 1 ? __float_as_uint(__ldg(p + 1)) : 0u, n > 2 ? __float_as_uint(__ldg(p + 2)) : 0u, 0u);
+    }
+};
+
+// A row is shared by WPR warps and stays in registers between the maximum and the quantisation, so it is read once: lane owns CPL
+// 16-byte chunks. Bound by HBM: 3 bytes a value for FP16.
+template <typename T, int CPL, int WPR>
+__global__ void __launch_bounds__(kThreads) quantizeRowsKernel(int64_t const rows, int32_t const width, T const* __restrict__ in,
+    int64_t const inStride, int8_t* __restrict__ out, int64_t const outStride, float* __restrict__ scales)
+{
+    constexpr int E = Chunk<T>::kElems;
+    constexpr int kRowsPerCta = kThreads / 32 / WPR;
+    __shared__ float red[kRowsPerCta][2][WPR];
+    int turn = 0;
+    int const lane = threadIdx.x & 31;
+    int const warp = threadIdx.x >> 5;
+    int const rowInCta = warp / WPR;
+    int const wInRow = warp % WPR;
+    gridDependencyLaunch();
+    gridDependencyWait();
+
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerCta + rowInCta; row < rows; row += static_cast<int64_t>(gridDim.x) * kRowsPerCta)
+    {
+        uint4 v[CPL];
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < CPL; ++i)
+        {
+            int const left = width - ((i * WPR + wInRow) * 32 + lane) * E;
+            T const* const p = in + row * inStride + ((i * WPR + wInRow) * 32 + lane) * E;
+            v[i] = left >= E ? ldgStream(p) : left > 0 ? Chunk<T>::loadPart(p, left) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < CPL; ++i)
+            m = maxNan(m, Chunk<T>::absMax(v[i]));
+        RowScale const s = makeRowScale(rowMax<WPR>(m, red[rowInCta], rowInCta, wInRow, lane, turn));
+        if (wInRow == 0 && lane == 0)
+            scales[row] = s.scale;
+#pragma unroll
+        for (int i = 0; i < CPL; ++i)
+        {
+            int const left = width - ((i * WPR + wInRow) * 32 + lane) * E;
+            int8_t* const p = out + row * outStride + ((i * WPR + wInRow) * 32 + lane) * E;
+            if (left <= 0)
+                continue;
+            float f[E];
+            Chunk<T>::unpack(v[i], f);
+            uint32_t w[E / 4];
+            quantRowChunk<E, sizeof(T) == 4>(f, s, w);
+            if (left >= E)
+            {
+                if constexpr (E == 8)
+                    stgStream8(p, make_uint2(w[0], w[1]));
+                else
+                    *reinterpret_cast<uint32_t*>(p) = w[0];
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (j < left)
+                        p[j] = static_cast<int8_t>(w[j / 4] >> (8 * (j & 3)));
+            }
+        }
+    }
+}
+
+// Rows longer than the registers of eight warps, or not aligned for wide accesses: a CTA per row reads it twice (the second time from
+// L1 or L2), one value per lane.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) quantizeRowsLongKernel(int64_t const rows, int32_t const width, T const* __restrict__ in,
+    int64_t const inStride, int8_t* __restrict__ out, int64_t const outStride, float* __restrict__ scales)
+{
+    __shared__ float red[2][kThreads / 32];
+    int turn = 0;
+    gridDependencyLaunch();
+    gridDependencyWait();
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
+    {
+        T const* const p = in + row * inStride;
+        float m = 0.f;
+#pragma unroll 8
+        for (int i = threadIdx.x; i < width; i += kThreads)
+            m = maxNan(m, fabsf(static_cast<float>(p[i])));
+        RowScale const s = makeRowScale(rowMax<kThreads / 32>(m, red, 0, threadIdx.x >> 5, threadIdx.x & 31, turn));
+        if (threadIdx.x == 0)
+            scales[row] = s.scale;
+#pragma unroll 8
+        for (int i = threadIdx.x; i < width; i += kThreads)
+            out[row * outStride + i] = quantRowValue<sizeof(T) == 4>(static_cast<float>(p[i]), s);
+    }
+}
+
+template <typename T>
+int32_t quantizeRows(cudaStream_t stream, int64_t rows, int32_t width, T const* in, int64_t inStride, int8_t* out, int64_t outStride, float* scales)
+{
+    constexpr int E = Chunk<T>::kElems;
+    int const chunks = (width + E - 1) / E;
+    bool const aligned = aligned16(in) && inStride % E == 0 && (reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(outStride)) % E == 0;
+    cudaError_t e = cudaErrorUnknown;
+    if (!aligned || chunks > 8 * 4 * 32)
+    {
+        int64_t const most = static_cast<int64_t>(smCount()) * 8;
+        e = launchDependent(quantizeRowsLongKernel<T>, dim3(static_cast<unsigned>(rows < most ? rows : most)), dim3(kThreads), 0, stream, rows, width, in,
+            inStride, out, outStride, scales);
+    }
+    else
+    {
+        int wpr = 1;
+        while (chunks > 32 * 4 * wpr)
+            wpr *= 2;
+        int const cpl = (chunks + 32 * wpr - 1) / (32 * wpr);
+        int64_t const ctas = (rows + 8 / wpr - 1) / (8 / wpr);
+        int64_t const most = static_cast<int64_t>(smCount()) * 8;
+        unsigned const grid = static_cast<unsigned>(ctas < most ? ctas : most);
+#define B200_QUANT_CASE(C, W)                                                                                          \
+    if (cpl == C && wpr == W)                                                                                          \
+        e = launchDependent(quantizeRowsKernel<T, C, W>, dim3(grid), dim3(kThreads), 0, stream, rows, width, in, inStride, out, outStride, scales);
+        B200_QUANT_CASE(1, 1)
+        B200_QUANT_CASE(2, 1)
+        B200_QUANT_CASE(3, 1)
+        B200_QUANT_CASE(4, 1)
+        B200_QUANT_CASE(3, 2)
+        B200_QUANT_CASE(4, 2)
+        B200_QUANT_CASE(3, 4)
+        B200_QUANT_CASE(4, 4)
+        B200_QUANT_CASE(3, 8)
+        B200_QUANT_CASE(4, 8)
+#undef B200_QUANT_CASE
+    }
+    if (e != cudaSuccess)
+        B200_FAIL(BERT_B200_CUDA_ERROR, "quantizeRowsKernel: %s", cudaGetErrorString(e));
+    return checkLaunch("quantizeRowsKernel");
+}
+
+} // namespace
+} // namespace b200
+
+using namespace b200;
+
+extern "C" int32_t bert_b200_quantize_rows(void* stream, int32_t type_id, int64_t rows, int32_t width, void const* input, int64_t input_stride,
+    int8_t* output, int64_t output_stride, float* row_scales)
+{
+    B200_REQUIRE(type_id == BERT_B200_FP16 || type_id == BERT_B200_FP32, "quantize_rows: type_id %d (FP16 or FP32)", type_id);
+    B200_REQUIRE(rows >= 0 && width > 0 && width <= 1 << 30, "quantize_rows: bad sizes rows=%lld width=%d", static_cast<long long>(rows), width);
+    B200_REQUIRE(input_stride >= width && output_stride >= width, "quantize_rows: a row stride is smaller than the row's %d values", width);
+    if (rows == 0)
+        return BERT_B200_OK;
+    B200_REQUIRE(input && output && row_scales, "quantize_rows: null pointer");
+    uintptr_t const elem = type_id == BERT_B200_FP16 ? 2 : 4;
+    B200_REQUIRE(reinterpret_cast<uintptr_t>(input) % elem == 0 && reinterpret_cast<uintptr_t>(row_scales) % 4 == 0,
+        "quantize_rows: input or row_scales is not aligned to its type");
+    auto s = static_cast<cudaStream_t>(stream);
+    if (type_id == BERT_B200_FP16)
+        return quantizeRows(s, rows, width, static_cast<__half const*>(input), input_stride, output, output_stride, row_scales);
+    return quantizeRows(s, rows, width, static_cast<float const*>(input), input_stride, output, output_stride, row_scales);
+}

@@ -7,6 +7,7 @@ libbert_b200.so. Names follow the reference free functions they replace
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -161,6 +162,135 @@ def fc(a, wt, bias=None, activation=ACT_NONE, alpha=1.0, out_dtype=None, out_sca
                       out.stride(0), _ptr(bias), activation, alpha, out_scale, _ptr(status))
     check(lib.bert_b200_fc(C.byref(p), _stream()), "fc")
     return out
+
+
+def _here(*tensors):
+    """The operators below run on the current device and its current stream; tensors of another device are refused."""
+    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            if not t.is_cuda:
+                raise ValueError("tensorrt_b200 kernels need CUDA tensors; there is no CPU path")
+            raise ValueError(f"tensor on {t.device}, which is not the current device")
+
+
+def _vector(t, n, what):
+    """Pointer of a contiguous FP32 vector of n values."""
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous float32 vector of {n} values, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _row_stride(t, what, multiple=1):
+    """Row stride of a matrix whose rows are contiguous (views of wider tensors are fine)."""
+    rows, width = t.shape
+    if width > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: the values of a row must be contiguous")
+    return t.stride(0) if rows > 1 else (width + multiple - 1) // multiple * multiple  # of a single row the stride says nothing
+
+
+def _int8_rows(rows, width, device):
+    """INT8 matrix whose rows begin on 16 bytes, as fc_rowwise reads it."""
+    t = torch.empty((rows, (width + 15) & ~15), dtype=torch.int8, device=device)
+    return t if width & 15 == 0 else t[:, :width]
+
+
+def quantize_rows(x):
+    """FP16/FP32 [..., width] -> (INT8 of the same shape, FP32 scale of each row): scale = max|row| / 127, values rounded to nearest even.
+    A matrix may be a view with a row stride. The INT8 rows begin on 16 bytes, so they are a view where the width is not a multiple of
+    16. Also makes per-channel weights for fc_rowwise out of an [n, k] weight. A row of zeros has scale 0, a row with NaN or infinity
+    scale NaN."""
+    _here(x)
+    if x.dtype not in (torch.float16, torch.float32):
+        raise ValueError(f"quantize_rows takes float16 or float32, not {x.dtype}")
+    if x.dim() != 2:
+        if x.dim() == 0 or not x.is_contiguous():
+            raise ValueError("quantize_rows: a tensor that is no matrix must be contiguous, with at least one dimension")
+        q, scales = quantize_rows(x.view(-1, x.shape[-1]))
+        return q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0], scales.view(x.shape[:-1])
+    rows, width = x.shape
+    q = _int8_rows(rows, width, x.device)
+    scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    check(lib.bert_b200_quantize_rows(_stream(), _TYPE_ID[x.dtype], rows, width, x.data_ptr(), _row_stride(x, "quantize_rows"), q.data_ptr(),
+                                      (width + 15) & ~15, scales.data_ptr()), "quantize_rows")
+    return q, scales
+
+
+def fc_rowwise(a, a_scales, wt, wt_scales, bias=None, activation=ACT_NONE, out_dtype=torch.float16, status=None, out=None):
+    """C[m, n] = act((A[m, k] . Wt[n, k]) * a_scales[m] * wt_scales[n] + bias[n]): INT8 operands as quantize_rows gives them, FP16 or FP32
+    result, any sizes. Rows of A, Wt and `out` begin on 16 bytes (they may be views of wider tensors); without `out`, a result whose rows would
+    not is a view of padded rows."""
+    _here(a, a_scales, wt, wt_scales, bias, status, out)
+    if a.dtype != torch.int8 or wt.dtype != torch.int8 or a.dim() != 2 or wt.dim() != 2 or a.shape[1] != wt.shape[1]:
+        raise ValueError(f"fc_rowwise takes int8 matrices [m, k] and [n, k], got {a.dtype} {tuple(a.shape)} and {wt.dtype} {tuple(wt.shape)}")
+    if out_dtype not in (torch.float16, torch.float32):
+        raise ValueError(f"fc_rowwise gives float16 or float32, not {out_dtype}")
+    m, k = a.shape
+    n = wt.shape[0]
+    per = 16 // out_dtype.itemsize
+    if out is None:
+        padded = (n + per - 1) // per * per
+        out = torch.empty((m, padded), dtype=out_dtype, device=a.device)
+        if padded != n:
+            out = out[:, :n]
+    elif out.dtype != out_dtype or tuple(out.shape) != (m, n):
+        raise ValueError(f"out must be a {out_dtype} tensor of shape {(m, n)}")
+    p = _lib.FcRowwiseParams(_TYPE_ID[out_dtype], activation, m, n, k, a.data_ptr(), _row_stride(a, "a", 16), _vector(a_scales, m, "a_scales"),
+                             wt.data_ptr(), _row_stride(wt, "wt", 16), _vector(wt_scales, n, "wt_scales"), out.data_ptr(),
+                             _row_stride(out, "out", per), None if bias is None else _vector(bias, n, "bias"), _ptr(status))
+    check(lib.bert_b200_fc_rowwise(C.byref(p), _stream()), "fc_rowwise")
+    return out
+
+
+def skip_layer_norm_quantize(x, skip, gamma, beta, bias=None, eps=0.0, with_output=True):
+    """Residual (+ bias) + LayerNorm over the last dimension whose result is also quantised row by row: (y, INT8 rows, FP32 scales). `skip` None:
+    LayerNorm alone; with_output False: y is None. y has the bits of skip_layer_norm (whose FP16 form has eps 0); the INT8 rows are those
+    of the FP32 result before it is rounded to y's type. They feed fc_rowwise where the width is a multiple of 16."""
+    _here(x, skip, gamma, beta, bias)
+    ld = x.shape[-1]
+    for t, shape, what in ((skip, x.shape, "skip"), (gamma, (ld,), "gamma"), (beta, (ld,), "beta"), (bias, (ld,), "bias")):
+        if t is not None and (t.dtype != x.dtype or t.shape != shape):
+            raise ValueError(f"skip_layer_norm_quantize: {what} must be {x.dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if x.dtype not in (torch.float16, torch.float32):
+        raise ValueError(f"skip_layer_norm_quantize takes float16 or float32, not {x.dtype}")
+    y = torch.empty_like(x) if with_output else None
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    check(lib.bert_b200_skip_layer_norm_quantize(_stream(), _TYPE_ID[x.dtype], ld, x.numel(), _ptr(x), _ptr(skip), _ptr(beta), _ptr(gamma), _ptr(y),
+                                                 q.data_ptr(), scales.data_ptr(), _ptr(bias), eps), "skip_layer_norm_quantize")
+    return y, q, scales
+
+
+class LogProbs(NamedTuple):
+    log_probs: torch.Tensor | None       # [rows, tokens]
+    entropy: torch.Tensor                # [rows]
+    top_ids: torch.Tensor | None         # [rows, top_k]
+    top_log_probs: torch.Tensor | None
+
+
+def token_log_probs(logits, token_ids=None, top_k=0):
+    """Log probabilities of given tokens, entropy and the top_k (at most 32) most likely tokens of each row of FP16/FP32 logits [rows, vocab], a
+    matrix or a view with a row stride. token_ids: int32 [rows, tokens] or [rows]; ids outside the vocabulary have probability 0. Tokens of
+    logit -inf are no alternatives (ids -1 where too few are left); rows with NaN or +inf give NaN."""
+    _here(logits, token_ids)
+    if logits.dtype not in (torch.float16, torch.float32) or logits.dim() != 2:
+        raise ValueError(f"token_log_probs takes float16 or float32 logits [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    tokens = 0
+    if token_ids is not None:
+        if token_ids.dtype != torch.int32 or token_ids.dim() not in (1, 2) or token_ids.shape[0] != rows or not token_ids.is_contiguous():
+            raise ValueError(f"token_ids must be a contiguous int32 tensor [{rows}, tokens] or [{rows}], got {token_ids.dtype} {tuple(token_ids.shape)}")
+        tokens = token_ids.shape[1] if token_ids.dim() == 2 else 1
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    lp = torch.empty(token_ids.shape, **f32) if token_ids is not None else None
+    entropy = torch.empty((rows,), **f32)
+    ids = torch.empty((rows, top_k), dtype=torch.int32, device=logits.device) if top_k > 0 else None
+    top = torch.empty((rows, top_k), **f32) if top_k > 0 else None
+    p = _lib.LogProbsParams(_TYPE_ID[logits.dtype], rows, vocab, logits.data_ptr(), _row_stride(logits, "token_log_probs"), tokens,
+                            token_ids.data_ptr() if tokens else None, top_k, lp.data_ptr() if tokens else None, entropy.data_ptr(),
+                            ids.data_ptr() if ids is not None else None, top.data_ptr() if top is not None else None)
+    check(lib.bert_b200_token_log_probs(C.byref(p), _stream()), "token_log_probs")
+    return LogProbs(lp, entropy, ids, top)
 
 
 def attention_bnsd(q, k, v, kv_lengths=None, scale_bmm1=None, scale_softmax=1.0, scale_bmm2=1.0, status=None):
