@@ -267,10 +267,9 @@ __device__ __forceinline__ float maxNan(float a, float b)
 
 __device__ __forceinline__ float warpMaxNan(float v)
 {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        v = maxNan(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    float m;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
 }
 
 // 128-bit global load through the read-only path, no L1 allocation (streamed once).

@@ -5,10 +5,13 @@
 // The maxima are kept out of s so that a row that is sure of a token keeps the digits of 1 - p: L is then as precise as s.
 // No counterpart in the reference (its plugins end at the encoder's output).
 //
-// A group of W warps takes a part of a row, NV 16-byte vectors per thread, into registers, so that the maximum is known before the first
-// exponential and nothing is read twice. The k most likely tokens: the k-th largest of 32 groups' maxima is a lower bound of the k-th
-// largest value, so only what is at least that (a few more than k) is listed and ranked, by value, then by the lower id. Rows where the
-// list overflows (thousands of equal values) are selected one after the other from the L2 instead.
+// A CTA takes a row (a part of it, where it is long) into shared memory by asynchronous copies, every thread the 16-byte vectors that it
+// will read itself, so the maximum is known before the first exponential and nothing is read twice; the next part's copies are on their
+// way as soon as a thread has read its vectors for the last time. W warps do that; one more puts the results together (it keeps the likely
+// tokens, a lane each, and writes what is asked for) while they are at the next part, from one of two hand-over places.
+// The k most likely tokens: the k-th largest of 32 groups' maxima is a lower bound of the k-th largest value, so only what is at least that
+// (a few more than k) is handed over. Where that is more than the list holds (hundreds of equal values) the last warp reads the part again.
+// Rows of up to 128 vectors: one warp each, the same steps one after the other.
 // Rows longer than a part: a cluster of CTAs takes the parts at once and joins them through distributed shared memory where that does not
 // take SMs from other rows; otherwise a CTA takes them by turns.
 #include "common.cuh"
@@ -74,12 +77,41 @@ struct Vec<__half>
     {
         unpackHalf8(v, f);
     }
+    // values below `floor` become it
+    static __device__ __forceinline__ void unpackAbove(uint4 const& v, float floor, float (&f)[8])
+    {
+        __half2 const* h = reinterpret_cast<__half2 const*>(&v);
+        __half2 const lo = __float2half2_rn(floor);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            float2 const t = __half22float2(__hmax2(h[i], lo));
+            f[2 * i] = t.x;
+            f[2 * i + 1] = t.y;
+        }
+    }
     static __device__ __forceinline__ float most(uint4 const& v)
     {
         __half2 const* h = reinterpret_cast<__half2 const*>(&v);
         __half2 const m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
         return maxNan(__low2float(m), __high2float(m));
     }
+    // the maximum of many vectors
+    struct Most
+    {
+        __half2 a = __half2half2(__ushort_as_half(0xfc00)), b = a;
+        __device__ __forceinline__ void add(uint4 const& v)
+        {
+            __half2 const* h = reinterpret_cast<__half2 const*>(&v);
+            a = __hmax2_nan(a, __hmax2_nan(h[0], h[1]));
+            b = __hmax2_nan(b, __hmax2_nan(h[2], h[3]));
+        }
+        __device__ __forceinline__ float get() const
+        {
+            __half2 const m = __hmax2_nan(a, b);
+            return maxNan(__low2float(m), __high2float(m));
+        }
+    };
 };
 template <>
 struct Vec<float>
@@ -92,23 +124,31 @@ struct Vec<float>
         f[2] = __uint_as_float(v.z);
         f[3] = __uint_as_float(v.w);
     }
+    static __device__ __forceinline__ void unpackAbove(uint4 const& v, float floor, float (&f)[4])
+    {
+        unpack(v, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            f[i] = fmaxf(f[i], floor);
+    }
     static __device__ __forceinline__ float most(uint4 const& v)
     {
         return maxNan(maxNan(__uint_as_float(v.x), __uint_as_float(v.y)), maxNan(__uint_as_float(v.z), __uint_as_float(v.w)));
     }
+    struct Most
+    {
+        float a = negInf(), b = negInf();
+        __device__ __forceinline__ void add(uint4 const& v)
+        {
+            a = maxNan(a, maxNan(__uint_as_float(v.x), __uint_as_float(v.y)));
+            b = maxNan(b, maxNan(__uint_as_float(v.z), __uint_as_float(v.w)));
+        }
+        __device__ __forceinline__ float get() const
+        {
+            return maxNan(a, b);
+        }
+    };
 };
-
-template <typename T, typename F>
-__device__ __forceinline__ int countIf(uint4 const& v, F const& f)
-{
-    float x[Vec<T>::kElems];
-    Vec<T>::unpack(v, x);
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < Vec<T>::kElems; ++j)
-        n += f(x[j]) ? 1 : 0;
-    return n;
-}
 
 // Maximum, how often it occurs, sum and weighted sum of the others (see above). count == 0: nothing yet.
 struct alignas(16) Stat
@@ -131,408 +171,618 @@ __device__ __forceinline__ Stat merge(Stat const& a, Stat const& b)
     return Stat{hi.m, hi.count, fmaf(w, n, hi.s), fmaf(w, fmaf(d, n, lo.t), hi.t)};
 }
 
+// What the warps that read a part hand over.
 template <int W>
-struct Scratch
+struct Place
 {
-    static constexpr int kCap = W == 1 ? 256 : 512;
+    static constexpr int kCap = W == 1 ? 128 : 256;
     uint64_t cand[kCap];
-    uint64_t top[kMaxTop];
-    uint64_t best[W];
-    Stat stat;
-    float groupMax[32];
-    float2 sums[W];
-    float threshold;
-    int32_t ties, listed, topCount;
-    int32_t bad; // a NaN or +infinity has been seen
+    float2 sums[W * 32]; // of each thread
+    float m;            // the part's maximum; -infinity: nothing in it, NaN or +infinity: the row has no distribution
+    int32_t ties;       // how often it occurs
+    int32_t listed;     // candidates, also those beyond kCap
 };
 
-template <int W>
-__device__ __forceinline__ void groupSync()
+__device__ __forceinline__ void copyAsync16(uint4* dst, void const* src, int bytes)
 {
-    if (W == 1)
-        __syncwarp();
-    else
-        __syncthreads();
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copyAsync16(uint4* dst, void const* src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
 }
 
-// One part of a row: vectors [first, first + T * NV) of `nVec`; `p` is the row's first value, `mis` values behind a 16-byte boundary.
-// Adds to sh.stat and sh.top.
-template <typename T, int W, int NV>
-__device__ __forceinline__ void takePart(Scratch<W>& sh, T const* p, int mis, int32_t vocab, int first, int nVec, int topK, int tid)
+// A row as 16-byte vectors: `p` its first value, `mis` values behind a 16-byte boundary, nVec vectors that hold some of its values.
+template <typename T>
+struct Row
+{
+    static constexpr int E = Vec<T>::kElems;
+    T const* p;
+    int mis, nVec;
+    bool firstRow, lastRow;
+
+    __device__ __forceinline__ Row(LogProbsArgs const& args, int64_t row)
+        : p(static_cast<T const*>(args.logits) + row * args.stride)
+        , mis(static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T)))
+        , nVec((args.vocab + mis + E - 1) / E)
+        , firstRow(row * args.stride < E)
+        , lastRow((args.rows - 1 - row) * args.stride < E)
+    {
+    }
+
+    // The vectors [begin, end) of `n` from `first` on that can be copied as they are: whole vectors, with which values of the rows beside this
+    // one may come along; where there may be none, at the ends of the matrix, the row's first and last vector by copyEdge.
+    __device__ __forceinline__ int begin(int first) const
+    {
+        return firstRow && first == 0 ? 1 : 0;
+    }
+    __device__ __forceinline__ int end(int first, int n) const
+    {
+        return lastRow && first + n == nVec ? n - 1 : n;
+    }
+    __device__ __forceinline__ T const* at(int first) const
+    {
+        return p - mis + static_cast<int64_t>(first) * E;
+    }
+
+    // Starts the copies of this thread's share of `n` vectors from `first` on, from its vector `i` on.
+    template <int kThreads>
+    __device__ __forceinline__ void copy(uint4* buf, int first, int n, int i, int tid, LogProbsArgs const& args) const
+    {
+        if (n == 0)
+            return;
+        T const* const q = at(first);
+        int const lo = begin(first), hi = end(first, n);
+#pragma unroll 4
+        for (; i < hi; i += kThreads)
+            if (i >= lo)
+                copyAsync16(buf + i, q + static_cast<int64_t>(i) * E);
+        if (tid == 0 && lo > 0 && hi > 0)
+            copyEdge(buf, 0, args);
+        if (hi < n && hi % kThreads == tid)
+            copyEdge(buf + hi, nVec - 1, args);
+    }
+
+    // A vector that holds values of the row only in part, and beside them perhaps nothing that may be read.
+    __device__ __forceinline__ void copyEdge(uint4* dst, int vec, LogProbsArgs const& args) const
+    {
+        int32_t const e0 = vec * E - mis;
+        int const left = args.vocab - e0;
+        if (e0 >= 0)
+            copyAsync16(dst, p + e0, left < E ? left * static_cast<int>(sizeof(T)) : 16);
+        else
+            for (int j = 0; j < E; ++j)
+                if (e0 + j >= 0 && j < left)
+                    reinterpret_cast<T*>(dst)[j] = __ldg(p + e0 + j);
+    }
+
+    // What of the copied vector is not the row's becomes -infinity.
+    __device__ __forceinline__ void trim(uint4* dst, int vec, int32_t vocab) const
+    {
+        int32_t const e0 = vec * E - mis;
+        if (e0 < 0 || e0 + E > vocab)
+            for (int j = 0; j < E; ++j)
+                if (e0 + j < 0 || e0 + j >= vocab)
+                    reinterpret_cast<T*>(dst)[j] = static_cast<T>(negInf());
+    }
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Sums over a thread's values of exp(x - m) and (x - m) exp(x - m), two of each.
+struct Sums
+{
+    uint64_t s = pack2(0.f, 0.f), t = pack2(0.f, 0.f);
+};
+
+// For any m.
+template <typename T>
+__device__ __forceinline__ void addExponentials(uint4 const& v, float m, Sums& sums)
+{
+    constexpr int E = Vec<T>::kElems;
+    float f[E];
+    Vec<T>::unpack(v, f);
+#pragma unroll
+    for (int j = 0; j < E; j += 2)
+    {
+        float const a = fmaxf(f[j] - m, -200.f), b = fmaxf(f[j + 1] - m, -200.f); // masked values: 0 times a finite number
+        uint64_t const e = pack2(exp2Approx(a * kLog2e), exp2Approx(b * kLog2e));
+        sums.s = add2(sums.s, e);
+        sums.t = fma2(e, pack2(a, b), sums.t);
+    }
+}
+
+// For m of moderate size: sums of 2^u and u 2^u with u = x log2(e) - c, c = m log2(e) as rounded. u is
+// rounded once, whatever m; how far c is from m log2(e), the same for all values, is put right in `finish`.
+// Moderate: m - 100, rounded to FP16, stays more than 88 below m.
+constexpr float kModerate = 4096.f;
+template <typename T>
+__device__ __forceinline__ void addPowers(uint4 const& v, float floor, uint64_t minusC, Sums& sums)
+{
+    constexpr int E = Vec<T>::kElems;
+    uint64_t const log2e = pack2(kLog2e, kLog2e);
+    float f[E];
+    Vec<T>::unpackAbove(v, floor, f); // masked values: 0 times a finite number
+#pragma unroll
+    for (int j = 0; j < E; j += 2)
+    {
+        uint64_t const u = fma2(pack2(f[j], f[j + 1]), log2e, minusC);
+        float a, b;
+        unpack2(u, a, b);
+        uint64_t const e = pack2(exp2Approx(a), exp2Approx(b));
+        sums.s = add2(sums.s, e);
+        sums.t = fma2(e, u, sums.t);
+    }
+}
+
+// Barriers of the CTA: among the reading warps, and the two hand-over places' full and free ones (reading warps and the last one).
+enum
+{
+    kBarRead = 1,
+    kBarFull = 2,
+    kBarFree = 4
+};
+template <int kThreads>
+__device__ __forceinline__ void barSync(int id)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+}
+template <int kThreads>
+__device__ __forceinline__ void barArrive(int id)
+{
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+}
+
+// Reads the part that lies in `buf` (n vectors, vector `first` of the row first) and leaves what it found in `place`. `claim` waits until the
+// place is free; afterwards its counters are 0. `next` starts the copy that takes the place of a vector which has been read for the last time.
+template <typename T, int W, typename F, typename G>
+__device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float* threshold, uint4* buf, Row<T> const& row, int32_t vocab, int first, int n,
+    int topK, int tid, F const& claim, G const& next)
 {
     constexpr int kThreads = W * 32;
     constexpr int E = Vec<T>::kElems;
     int const lane = tid & 31, warp = tid >> 5;
-    uint4 v[NV];
-    uint32_t const fill = sizeof(T) == 2 ? 0xfc00fc00u : 0xff800000u; // -infinity
-    auto load = [&](int vec) {
-        int32_t const e0 = vec * E - mis;
-        if (e0 >= 0 && e0 + E <= vocab)
-            return ldgStream(p + e0);
-        uint4 r = make_uint4(fill, fill, fill, fill);
-        T* const e = reinterpret_cast<T*>(&r);
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (e0 + j >= 0 && e0 + j < vocab)
-                e[j] = __ldg(p + e0 + j);
-        return r;
+    auto sync = [&]() {
+        if (W == 1)
+            __syncwarp();
+        else
+            barSync<kThreads>(kBarRead);
     };
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (first + i * kThreads < nVec) // the same for all threads
-            v[i] = load(first + i * kThreads + tid);
-    float mine = negInf();
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (first + i * kThreads < nVec)
-            mine = maxNan(mine, Vec<T>::most(v[i]));
-    float g = mine;
-#pragma unroll
-    for (int o = 1; o < W; o *= 2)
-        g = maxNan(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if (lane % W == 0)
-        sh.groupMax[tid / W] = g;
-    // the tokens found so far compete with this part's
-    int const had = sh.topCount;
-    if (tid < had)
-        sh.cand[tid] = sh.top[tid];
-    groupSync<W>();
+    if (first == 0 && tid == 0)
+        row.trim(buf, 0, vocab);
+    if (first + n == row.nVec && (n - 1) % kThreads == tid)
+        row.trim(buf + n - 1, row.nVec - 1, vocab);
 
-    float const gm = sh.groupMax[lane];
+    typename Vec<T>::Most most;
+#pragma unroll 4
+    for (int i = tid; i < n; i += kThreads)
+        most.add(buf[i]);
+    float const mine = most.get();
+    float gm = mine;
+    if constexpr (W > 1)
+    {
+#pragma unroll
+        for (int o = 1; o < W; o *= 2)
+            gm = maxNan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+        if (lane % W == 0)
+            groupMax[tid / W] = gm;
+        claim();
+        sync();
+        gm = groupMax[lane];
+    }
     float const m = warpMaxNan(gm);
-    bool const bad = !(m < __int_as_float(0x7f800000)); // NaN or +infinity
-    bool const some = !bad && m != negInf();
+    bool const some = m < __int_as_float(0x7f800000) && m != negInf();
     if (tid == 0)
-        sh.bad |= bad ? 1 : 0;
-    float s = 0.f, t = 0.f;
-    if (some)
-    {
-        if (topK > 0 && warp == W - 1)
-        {
-            int rank = 0;
-#pragma unroll
-            for (int o = 1; o < 32; ++o)
-            {
-                float const x = __shfl_xor_sync(0xffffffffu, gm, o);
-                rank += x > gm || (x == gm && (lane ^ o) < lane) ? 1 : 0;
-            }
-            float thr = __shfl_sync(0xffffffffu, gm, __ffs(__ballot_sync(0xffffffffu, rank == topK - 1)) - 1);
-            if (had == topK)
-                thr = fmaxf(thr, keyValue(sh.cand[topK - 1]));
-            if (lane == 0)
-                sh.threshold = thr;
-        }
-        if (mine == m)
-        {
-            // the row's maxima are listed and counted here, and no longer among the others
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (first + i * kThreads < nVec)
-                    n += countIf<T>(v[i], [&](float x) { return x == m; });
-            atomicAdd(&sh.ties, n);
-            int at = topK > 0 ? atomicAdd(&sh.listed, n) : 0;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (first + i * kThreads < nVec)
-                {
-                    T* const e = reinterpret_cast<T*>(&v[i]);
-#pragma unroll
-                    for (int j = 0; j < E; ++j)
-                        if (static_cast<float>(e[j]) == m)
-                        {
-                            e[j] = static_cast<T>(negInf());
-                            if (topK > 0 && at < Scratch<W>::kCap)
-                                sh.cand[at++] = makeKey(m, (first + i * kThreads + tid) * E - mis + j);
-                        }
-                }
-        }
-        uint64_t const negM = pack2(-m, -m), log2e = pack2(1.4426950408889634f, 1.4426950408889634f);
-        uint64_t s2 = pack2(0.f, 0.f), t2 = s2;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (first + i * kThreads < nVec)
-            {
-                float f[E];
-                Vec<T>::unpack(v[i], f);
-#pragma unroll
-                for (int j = 0; j < E; j += 2)
-                {
-                    float a, b;
-                    unpack2(add2(pack2(f[j], f[j + 1]), negM), a, b);
-                    a = fmaxf(a, -200.f); // masked values: 0 times a finite number
-                    b = fmaxf(b, -200.f);
-                    uint64_t const d = pack2(a, b);
-                    unpack2(mul2(d, log2e), a, b);
-                    uint64_t const e = pack2(exp2Approx(a), exp2Approx(b));
-                    s2 = add2(s2, e);
-                    t2 = fma2(e, d, t2);
-                }
-            }
-        float a, b;
-        unpack2(s2, a, b);
-        s = a + b;
-        unpack2(t2, a, b);
-        t = a + b;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-    {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        t += __shfl_xor_sync(0xffffffffu, t, o);
-    }
-    if (lane == 0)
-        sh.sums[warp] = make_float2(s, t);
-    groupSync<W>();
-
-    if (some)
-    {
-        if (topK > 0)
-        {
-            float const thr = sh.threshold;
-            if (mine >= thr && mine != negInf())
-            {
-int n = 0;
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (first + i * kThreads < nVec)
-                        n += countIf<T>(v[i], [&](float x) { return x >= thr && x != negInf(); });
-                int at = atomicAdd(&sh.listed, n);
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (first + i * kThreads < nVec)
-                    {
-                        float f[E];
-                        Vec<T>::unpack(v[i], f);
-#pragma unroll
-                        for (int j = 0; j < E; ++j)
-                            if (f[j] >= thr && f[j] != negInf() && at < Scratch<W>::kCap)
-                                sh.cand[at++] = makeKey(f[j], (first + i * kThreads + tid) * E - mis + j);
-                    }
-            }
-        }
-        if (warp == 0)
-        {
-            float2 const x = lane < W ? sh.sums[lane] : make_float2(0.f, 0.f);
-            s = x.x;
-            t = x.y;
-#pragma unroll
-            for (int o = W / 2; o > 0; o >>= 1)
-            {
-                s += __shfl_xor_sync(0xffffffffu, s, o);
-                t += __shfl_xor_sync(0xffffffffu, t, o);
-            }
-            if (lane == 0)
-                sh.stat = merge(sh.stat, Stat{m, static_cast<float>(sh.ties), s, t});
-        }
-    }
-    groupSync<W>();
-
+        place.m = m;
+    float thr = m;
     if (some && topK > 0)
     {
-        int const n = sh.listed;
-        if (n <= Scratch<W>::kCap)
+        if constexpr (W == 1)
         {
-            for (int i = tid; i < n; i += kThreads)
-            {
-                uint64_t const k = sh.cand[i];
-                int rank = 0;
-                for (int j = 0; j < n; ++j)
-                    rank += sh.cand[j] > k ? 1 : 0;
-                if (rank < topK)
-                    sh.top[rank] = k;
-            }
-            if (tid == 0)
-                sh.topCount = n < topK ? n : topK;
+            // the largest is taken out topK - 1 times
+            float rest = gm;
+            for (int j = 1; j < topK; ++j)
+                if (__ffs(__ballot_sync(0xffffffffu, rest == warpMaxNan(rest))) - 1 == lane)
+                    rest = negInf();
+            thr = warpMaxNan(rest);
         }
         else
         {
-            // more than the list holds: the largest key that is below the last one found, topK times
-            uint64_t last = ~0ull;
-            auto scan = [&]() {
-                uint64_t best = tid < had && sh.cand[tid] < last ? sh.cand[tid] : 0ull;
-                for (int i = 0; i < NV; ++i)
-                    for (int j = 0; j < E; ++j)
-                    {
-                        int32_t const id = (first + i * kThreads + tid) * E - mis + j;
-                        if (id < 0 || id >= vocab)
-                            continue;
-                        float const x = static_cast<float>(__ldg(p + id));
-                        uint64_t const k = x == negInf() ? 0ull : makeKey(x, id);
-                        best = k < last && k > best ? k : best;
-                    }
-                return best;
-            };
-            uint64_t best = scan();
-            int found = 0;
-            for (; found < topK; ++found)
+            // the groups' maxima in order: each warp places 32 / W of them
+#pragma unroll
+            for (int j = 0; j < 32 / W; ++j)
             {
-                uint64_t k = best;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1)
-                {
-                    uint64_t const x = __shfl_xor_sync(0xffffffffu, k, o);
-                    k = x > k ? x : k;
-                }
-                if (lane == 0)
-                    sh.best[warp] = k;
-                groupSync<W>();
-                k = sh.best[0];
-#pragma unroll
-                for (int w = 1; w < W; ++w)
-                    k = sh.best[w] > k ? sh.best[w] : k;
-                groupSync<W>();
-                if (k == 0ull)
-                    break;
-                if (tid == 0)
-                    sh.top[found] = k;
-                if (best == k)
-                {
-                    last = k;
-                    best = scan();
-                }
+                int const at = warp * (32 / W) + j;
+                float const x = groupMax[at];
+                int const rank = __popc(__ballot_sync(0xffffffffu, gm > x || (gm == x && lane < at)));
+                if (rank == topK - 1 && lane == 0)
+                    *threshold = x;
             }
-            if (tid == 0)
-                sh.topCount = found;
         }
     }
-    if (tid == 0)
-        sh.ties = 0;
-    groupSync<W>();
-    if (tid == 0)
-        sh.listed = sh.topCount;
+    sync();
+    if (some)
+    {
+        if (W > 1 && topK > 0)
+            thr = *threshold;
+        // The warp looks through the vectors of its threads that have such values, a thread's at a time, two lanes per vector: candidates are
+        // listed; the part's maxima are counted and no longer among the others.
+        uint32_t hits = __ballot_sync(0xffffffffu, mine >= thr && mine != negInf());
+        for (; hits != 0; hits &= hits - 1)
+            for (int i = warp * 32 + __ffs(hits) - 1 + (lane >> 1) * kThreads; i < n; i += 16 * kThreads)
+            {
+                T* const e = reinterpret_cast<T*>(buf + i) + (lane & 1) * (E / 2);
+                uint2 const half = *reinterpret_cast<uint2 const*>(e);
+                if (Vec<T>::most(make_uint4(half.x, half.y, half.x, half.y)) < thr)
+                    continue;
+                for (int j = 0; j < E / 2; ++j)
+                {
+                    float const x = static_cast<float>(e[j]);
+                    if (x >= thr && x != negInf())
+                    {
+                        if (topK > 0)
+                        {
+                            int const at = atomicAdd(&place.listed, 1);
+                            if (at < Place<W>::kCap)
+                                place.cand[at] = makeKey(x, (first + i) * E - row.mis + (lane & 1) * (E / 2) + j);
+                        }
+                        if (x == m)
+                        {
+                            e[j] = static_cast<T>(negInf());
+                            atomicAdd(&place.ties, 1);
+                        }
+                    }
+                }
+            }
+        __syncwarp();
+    }
+    Sums sums;
+    float a, b, s, t;
+    if (fabsf(m) < kModerate)
+    {
+        float const c = m * kLog2e;
+        uint64_t const minusC = pack2(-c, -c);
+        float const floor = m - 100.f; // exp(-100) is below what FP32 holds in normal numbers
+#pragma unroll 4
+        for (int i = tid; i < n; i += kThreads)
+        {
+            addPowers<T>(buf[i], floor, minusC, sums);
+            next(i);
+        }
+        unpack2(sums.s, a, b);
+        s = a + b;
+        unpack2(sums.t, a, b);
+        t = a + b;
+        float const off = fmaf(m, kLog2e, -c), w = exp2Approx(-off); // u of m itself
+        t = fmaf(-off, s, t) * (w * 0.69314718055994531f);
+        s *= w;
+    }
+    else
+    {
+        for (int i = tid; i < n; i += kThreads)
+        {
+            if (some)
+                addExponentials<T>(buf[i], m, sums);
+            next(i);
+        }
+        unpack2(sums.s, a, b);
+        s = a + b;
+        unpack2(sums.t, a, b);
+        t = a + b;
+    }
+    place.sums[tid] = make_float2(s, t);
 }
 
-// kRows rows per CTA (one per warp) where W == 1; otherwise one row per cluster of `gridDim.x / rows` CTAs.
-template <typename T, int W, int NV, int kRows>
-__global__ void __launch_bounds__(W * 32 * kRows, W == 16 ? 2 : 1) logProbsKernel(LogProbsArgs const args, int const clusterSize)
+// A row's results as one warp collects them.
+struct Result
 {
-    static_assert(W == 1 || kRows == 1, "several rows per CTA: one warp each");
-    constexpr int kThreads = W * 32;
-    constexpr int E = Vec<T>::kElems;
-    __shared__ Scratch<W> scratch[kRows];
-    int const tid = W == 1 ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
-    Scratch<W>& sh = scratch[W == 1 ? threadIdx.x >> 5 : 0];
-    int const rank = W == 1 ? 0 : static_cast<int>(blockIdx.x % clusterSize);
-    int64_t const row = W == 1 ? static_cast<int64_t>(blockIdx.x) * kRows + (threadIdx.x >> 5) : static_cast<int64_t>(blockIdx.x / clusterSize);
-    gridDependencyLaunch();
-    if (tid == 0)
-    {
-        sh.stat = Stat{negInf(), 0.f, 0.f, 0.f};
-        sh.ties = sh.listed = sh.topCount = sh.bad = 0;
-    }
-    gridDependencyWait();
-    if (row >= args.rows) // whole warps of a CTA that has no other barrier
-        return;
-    groupSync<W>();
-    T const* const p = static_cast<T const*>(args.logits) + row * args.stride;
-    int const mis = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
-    int const nVec = (args.vocab + mis + E - 1) / E;
-    // the tokens asked for: their logits are on the way while the row is worked on
-    int32_t token = -1;
-    float tokenLogit = negInf();
-    if (rank == 0 && tid < args.numTokens)
-    {
-        token = __ldg(args.tokenIds + row * args.numTokens + tid);
-        if (token >= 0 && token < args.vocab)
-            tokenLogit = static_cast<float>(__ldg(p + token));
-    }
-    for (int first = rank * kThreads * NV; first < nVec; first += clusterSize * kThreads * NV)
-        takePart<T, W, NV>(sh, p, mis, args.vocab, first, nVec, args.topK, tid);
+    Stat stat{negInf(), 0.f, 0.f, 0.f};
+    uint64_t key = 0; // of this lane's place among the likely tokens, 0: none
+    bool bad = false; // a NaN or +infinity has been seen
 
-    if (W > 1 && clusterSize > 1)
+    // One key per lane (0: none) to the likely tokens.
+    __device__ __forceinline__ void insert(uint64_t k, int topK, int lane)
     {
-        clusterBarrier();
-        if (rank == 0)
+        uint32_t todo = __ballot_sync(0xffffffffu, k > __shfl_sync(0xffffffffu, key, topK - 1));
+        for (; todo != 0; todo &= todo - 1)
         {
-            // what the other CTAs found, joined by this one: their sums in order, their tokens ranked together
-            Stat st = sh.stat;
-            int bad = sh.bad, n = sh.topCount;
-            for (int i = tid; i < n; i += kThreads)
-                sh.cand[i] = sh.top[i];
-            for (int r = 1; r < clusterSize; ++r)
-            {
-                float4 const x = ldSharedCluster4(reinterpret_cast<float const*>(&sh.stat), r);
-                st = merge(st, Stat{x.x, x.y, x.z, x.w});
-                bad |= static_cast<int>(ldSharedCluster(reinterpret_cast<uint32_t const*>(&sh.bad), r));
-                int const more = static_cast<int>(ldSharedCluster(reinterpret_cast<uint32_t const*>(&sh.topCount), r));
-                if (tid < more)
-                {
-                    uint32_t const* const k = reinterpret_cast<uint32_t const*>(&sh.top[tid]);
-                    sh.cand[n + tid] = static_cast<uint64_t>(ldSharedCluster(k + 1, r)) << 32 | ldSharedCluster(k, r);
-                }
-                n += more;
-            }
-            __syncthreads();
-            if (tid == 0)
-            {
-                sh.stat = st;
-                sh.bad = bad;
-                sh.topCount = n < args.topK ? n : args.topK;
-            }
-            for (int i = tid; i < n; i += kThreads)
-            {
-                uint64_t const k = sh.cand[i];
-                int place = 0;
-                for (int j = 0; j < n; ++j)
-                    place += sh.cand[j] > k ? 1 : 0;
-                if (place < args.topK)
-                    sh.top[place] = k;
-            }
-            __syncthreads();
+            uint64_t const x = __shfl_sync(0xffffffffu, k, __ffs(todo) - 1);
+            int const at = __popc(__ballot_sync(0xffffffffu, key > x));
+            uint64_t const before = __shfl_up_sync(0xffffffffu, key, 1);
+            key = lane < at ? key : lane == at ? x : before;
         }
-        clusterBarrier(); // the others' shared memory has been read
-        if (rank != 0)
-            return;
     }
-    groupSync<W>();
+};
 
-    Stat const st = sh.stat;
-    bool const bad = sh.bad != 0;
+// Adds what is in `place` to the result and empties the place.
+template <typename T, int W>
+__device__ __forceinline__ void takePlace(Result& res, Place<W>& place, Row<T> const& row, int32_t vocab, int first, int n, int topK, int lane)
+{
+    constexpr int E = Vec<T>::kElems;
+    float const m = place.m;
+    if (!(m < __int_as_float(0x7f800000)))
+        res.bad = true;
+    else if (m != negInf())
+    {
+        float s = 0.f, t = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+        {
+            float2 const x = place.sums[w * 32 + lane];
+            s += x.x;
+            t += x.y;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+        {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            t += __shfl_xor_sync(0xffffffffu, t, o);
+        }
+        res.stat = merge(res.stat, Stat{m, static_cast<float>(place.ties), s, t});
+        int const listed = topK > 0 ? place.listed : 0;
+        if (listed <= Place<W>::kCap)
+            for (int i = 0; i < listed; i += 32)
+                res.insert(i + lane < listed ? place.cand[i + lane] : 0ull, topK, lane);
+        else
+        {
+            int32_t const begin = max(first * E - row.mis, 0), end = min((first + n) * E - row.mis, vocab);
+            for (int32_t i = begin; i < end; i += 32)
+            {
+                float const v = i + lane < end ? static_cast<float>(__ldg(row.p + i + lane)) : negInf();
+                res.insert(v == negInf() ? 0ull : makeKey(v, i + lane), topK, lane);
+            }
+        }
+    }
+    __syncwarp();
+    if (lane == 0)
+        place.ties = place.listed = 0;
+}
+
+// Writes a row's answers. `tokenLogit`: that of token `lane` of the first 32.
+template <typename T>
+__device__ __forceinline__ void writeRow(LogProbsArgs const& args, Result const& res, Row<T> const& row, int64_t r, float tokenLogit, int lane)
+{
+    Stat const& st = res.stat;
+    bool const bad = res.bad;
     bool const none = !bad && st.count == 0.f;
     float const nan = __int_as_float(0x7fffffff);
     float const lse = none ? 0.f : logf(st.count) + log1pf(st.s / st.count);
     auto logProb = [&](float x) {
         return bad ? nan : none ? negInf() : (x - st.m) - lse;
     };
-    for (int j = tid; j < args.numTokens; j += kThreads)
+    if (lane < args.numTokens)
+        args.logProbs[r * args.numTokens + lane] = logProb(tokenLogit);
+#pragma unroll 4
+    for (int j = lane + 32; j < args.numTokens; j += 32)
     {
-        if (j != tid)
-        {
-            token = __ldg(args.tokenIds + row * args.numTokens + j);
-            tokenLogit = token >= 0 && token < args.vocab ? static_cast<float>(__ldg(p + token)) : negInf();
-        }
-        args.logProbs[row * args.numTokens + j] = logProb(tokenLogit);
+        int32_t const token = __ldg(args.tokenIds + r * args.numTokens + j);
+        float const x = token >= 0 && token < args.vocab ? static_cast<float>(__ldg(row.p + token)) : negInf();
+        args.logProbs[r * args.numTokens + j] = logProb(x);
     }
-    if (tid == 0 && args.entropy)
-        args.entropy[row] = bad ? nan : none ? 0.f : lse - st.t / (st.count + st.s);
-    if (tid < args.topK)
+    if (lane == 0 && args.entropy)
+        args.entropy[r] = bad ? nan : none ? 0.f : lse - st.t / (st.count + st.s);
+    if (lane < args.topK)
     {
-        bool const have = !bad && tid < sh.topCount;
-        uint64_t const k = have ? sh.top[tid] : 0ull;
-        args.topIds[row * args.topK + tid] = have ? keyId(k) : -1;
-        args.topLogProbs[row * args.topK + tid] = have ? logProb(keyValue(k)) : bad ? nan : negInf();
+        bool const have = !bad && res.key != 0;
+        args.topIds[r * args.topK + lane] = have ? keyId(res.key) : -1;
+        args.topLogProbs[r * args.topK + lane] = have ? logProb(keyValue(res.key)) : bad ? nan : negInf();
     }
 }
 
+// The logit of token `lane` of the first 32 asked for.
+template <typename T>
+__device__ __forceinline__ float loadToken(LogProbsArgs const& args, Row<T> const& row, int64_t r, int lane)
+{
+    if (lane < args.numTokens)
+    {
+        int32_t const token = __ldg(args.tokenIds + r * args.numTokens + lane);
+        if (token >= 0 && token < args.vocab)
+            return static_cast<float>(__ldg(row.p + token));
+    }
+    return negInf();
+}
+
+__device__ __forceinline__ void copiesWait()
+{
+    asm volatile("cp.async.wait_all;" ::: "memory"); // every thread reads its own copies (or, behind a warp's barrier, its warp's)
+}
+
+// Short rows: a warp each, kGroups of them per CTA. `partVecs`: vectors of a row, at most.
+template <typename T, int kGroups>
+__global__ void __launch_bounds__(32 * kGroups) logProbsWarpKernel(LogProbsArgs const args, int const partVecs)
+{
+    __shared__ Place<1> places[kGroups];
+    extern __shared__ __align__(16) uint4 buffers[];
+    int const lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+    Place<1>& place = places[group];
+    uint4* const buf = buffers + group * partVecs;
+    int64_t const rowStep = static_cast<int64_t>(gridDim.x) * kGroups;
+    if (lane == 0)
+        place.ties = place.listed = 0;
+    gridDependencyLaunch();
+    gridDependencyWait();
+    int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+    if (r < args.rows)
+    {
+        Row<T> const row(args, r);
+        row.template copy<32>(buf, 0, row.nVec, lane, lane, args);
+    }
+    for (; r < args.rows; r += rowStep)
+    {
+        Row<T> const row(args, r);
+        float const tokenLogit = loadToken(args, row, r, lane);
+        copiesWait();
+        Result res;
+        readPart<T, 1>(place, nullptr, nullptr, buf, row, args.vocab, 0, row.nVec, args.topK, lane, []() {}, [](int) {});
+        if (r + rowStep < args.rows)
+        {
+            Row<T> const next(args, r + rowStep);
+            next.template copy<32>(buf, 0, next.nVec, lane, lane, args);
+        }
+        __syncwarp();
+        takePlace<T, 1>(res, place, row, args.vocab, 0, row.nVec, args.topK, lane);
+        writeRow(args, res, row, r, tokenLogit, lane);
+    }
+}
+
+// Rows are dealt over clusters of `clusterSize` CTAs, of which a CTA takes every clusterSize-th part of `partVecs` vectors.
+template <typename T, int W>
+__global__ void __launch_bounds__((W + 1) * 32, 3) logProbsKernel(LogProbsArgs const args, int const clusterSize, int const partVecs)
+{
+    constexpr int kReaders = W * 32, kAll = kReaders + 32;
+    constexpr int E = Vec<T>::kElems;
+    __shared__ Place<W> places[2];
+    __shared__ float groupMax[32], threshold;
+    __shared__ Stat joinStat; // of this CTA, read by the cluster's first
+    __shared__ uint64_t joinTop[kMaxTop];
+    __shared__ uint32_t joinBad;
+    extern __shared__ __align__(16) uint4 buf[];
+    int const tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+    int const rank = static_cast<int>(blockIdx.x % clusterSize);
+    int64_t const rowStep = gridDim.x / clusterSize;
+    int const partStep = clusterSize * partVecs;
+    if (tid < 2)
+        places[tid].ties = places[tid].listed = 0;
+    gridDependencyLaunch();
+    __syncthreads();
+    gridDependencyWait();
+
+    int use = 0; // parts of this CTA so far
+    if (warp < W)
+    {
+        int64_t r = blockIdx.x / clusterSize;
+        int first = rank * partVecs;
+        auto vectors = [&](Row<T> const& row, int from) {
+            int const left = row.nVec - from;
+            return left < partVecs ? left > 0 ? left : 0 : partVecs;
+        };
+        if (r < args.rows)
+        {
+            Row<T> const row(args, r);
+            row.template copy<kReaders>(buf, first, vectors(row, first), tid, tid, args);
+        }
+        for (; r < args.rows; r += rowStep, first = rank * partVecs)
+        {
+            Row<T> const row(args, r);
+            bool const rowsLeft = r + rowStep < args.rows;
+            Row<T> const below(args, rowsLeft ? r + rowStep : r);
+            int n = vectors(row, first);
+            if (n == 0 && rowsLeft) // nothing of this row is this CTA's; of the next one it may be
+                below.template copy<kReaders>(buf, first, vectors(below, first), tid, tid, args);
+            while (n > 0)
+            {
+                // what comes after this part
+                bool const sameRow = first + partStep < row.nVec;
+                Row<T> const then = sameRow ? row : below;
+                int const thenFirst = sameRow ? first + partStep : rank * partVecs;
+                int const thenN = sameRow || rowsLeft ? vectors(then, thenFirst) : 0;
+                int const lo = then.begin(thenFirst), hi = thenN > 0 ? then.end(thenFirst, thenN) : 0;
+                T const* const q = then.at(thenFirst);
+                copiesWait();
+                readPart<T, W>(
+                    places[use & 1], groupMax, &threshold, buf, row, args.vocab, first, n, args.topK, tid,
+                    [&]() {
+                        if (use >= 2)
+                            barSync<kAll>(kBarFree + (use & 1));
+                    },
+                    [&](int i) {
+                        if (i >= lo && i < hi)
+                            copyAsync16(buf + i, q + static_cast<int64_t>(i) * E);
+                    });
+                barArrive<kAll>(kBarFull + (use & 1));
+                if (thenN > 0) // what lies beyond this part's vectors, and the edges
+                    then.template copy<kReaders>(buf, thenFirst, thenN, n <= tid ? tid : tid + (n - 1 - tid) / kReaders * kReaders + kReaders, tid, args);
+                ++use;
+                first = thenFirst;
+                n = sameRow ? thenN : 0;
+            }
+            if (clusterSize > 1)
+            {
+                clusterBarrier();
+                clusterBarrier();
+            }
+        }
+        for (int i = use < 2 ? 0 : use - 2; i < use; ++i) // the places' last releases
+            barSync<kAll>(kBarFree + (i & 1));
+        return;
+    }
+
+    for (int64_t r = blockIdx.x / clusterSize; r < args.rows; r += rowStep)
+    {
+        Row<T> const row(args, r);
+        float const tokenLogit = rank == 0 ? loadToken(args, row, r, lane) : negInf();
+        Result res;
+        for (int first = rank * partVecs; first < row.nVec; first += partStep, ++use)
+        {
+            int const n = row.nVec - first < partVecs ? row.nVec - first : partVecs;
+            barSync<kAll>(kBarFull + (use & 1));
+            takePlace<T, W>(res, places[use & 1], row, args.vocab, first, n, args.topK, lane);
+            __syncwarp();
+            barArrive<kAll>(kBarFree + (use & 1));
+        }
+        if (clusterSize > 1)
+        {
+            if (lane == 0)
+            {
+                joinStat = res.stat;
+                joinBad = res.bad ? 1u : 0u;
+            }
+            joinTop[lane] = res.key;
+            __syncwarp();
+            clusterBarrier();
+            if (rank == 0)
+                for (int c = 1; c < clusterSize; ++c)
+                {
+                    float4 const x = ldSharedCluster4(reinterpret_cast<float const*>(&joinStat), c);
+                    res.stat = merge(res.stat, Stat{x.x, x.y, x.z, x.w});
+                    res.bad |= ldSharedCluster(&joinBad, c) != 0;
+                    uint32_t const* const k = reinterpret_cast<uint32_t const*>(&joinTop[lane]);
+                    if (args.topK > 0)
+                        res.insert(static_cast<uint64_t>(ldSharedCluster(k + 1, c)) << 32 | ldSharedCluster(k, c), args.topK, lane);
+                }
+            clusterBarrier(); // the others' shared memory has been read
+        }
+        if (rank == 0)
+            writeRow(args, res, row, r, tokenLogit, lane);
+    }
+}
+
+constexpr int kReadingWarps = 8;
+constexpr int kCtasPerSm = 3;
+constexpr int kPartVecs = 4096; // 64 KB, so that three CTAs fit an SM
+
+// Which kernel, and how many CTAs share a row.
+//  - A warp per row for up to 64 vectors, and for up to 512 where there are rows for many warps: FP16 20000 x 2000 47 us against 118 us with
+//    a CTA per row, 10000 x 4000 35 / 65 us, but 600 x 4000 11.7 / 8.1 us and 100 x 2000 7.0 / 4.8 us; beyond 512, 5000 x 9000 61 / 40 us.
+//  - Two or four CTAs per row while all of them find a place at once and each has at least half a part: FP32 100 x 120000 36 us with one,
+//    23 with two, 17 with four; 200 x 30522 12.6 / 11.3 / 16.9 us; FP16 1 x 30522 6.0 / 5.9 / 6.7 us, 100 x 9000 5.5 / 6.6 / 8.0 us. Eight are
+//    placed late (100 x 30522 FP32 26 us), and so are clusters beyond what fits (640 x 30522 FP32 60 us with two, 28.5 us with one).
 template <typename T>
 int32_t launchLogProbs(LogProbsArgs const& args, cudaStream_t stream)
 {
     constexpr int E = Vec<T>::kElems;
-    int64_t const vecs = (static_cast<int64_t>(args.vocab) + E - 1) / E + 1; // a row may begin inside a vector
+    int const vecs = (args.vocab + E - 1) / E + 1; // a row may begin inside a vector
+    int64_t const sms = smCount();
     cudaError_t e;
-    if (vecs <= 32 * 4)
-        e = launchDependent(logProbsKernel<T, 1, 4, 4>, dim3(static_cast<unsigned>((args.rows + 3) / 4)), dim3(128), 0, stream, args, 1);
-    else if (vecs <= 256 * 4)
-        e = launchDependent(logProbsKernel<T, 8, 4, 1>, dim3(static_cast<unsigned>(args.rows)), dim3(256), 0, stream, args, 1);
+    if (vecs <= 64 || (vecs <= 512 && args.rows > 8 * sms))
+    {
+        constexpr int kGroups = 4;
+        static SmemOptIn optIn;
+        int64_t const most = sms * 16, ctas = (args.rows + kGroups - 1) / kGroups;
+        e = launchDependentCluster(&optIn, logProbsWarpKernel<T, kGroups>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(32 * kGroups),
+            static_cast<size_t>(vecs) * 16 * kGroups, stream, 1, args, vecs);
+    }
     else
     {
-        int64_t const resident = static_cast<int64_t>(smCount()) * 2;
+        static SmemOptIn optIn;
         int cluster = 1;
-        while (cluster < 8 && args.rows * cluster * 2 <= resident && vecs > 512 * cluster)
+        while (cluster < 4 && args.rows * cluster * 2 <= sms * kCtasPerSm && vecs > kPartVecs / 2 * cluster)
             cluster *= 2;
-        e = launchDependentCluster(nullptr, logProbsKernel<T, 16, 8, 1>, dim3(static_cast<unsigned>(args.rows * cluster)), dim3(512), 0, stream, cluster,
-            args, cluster);
+        int const share = (vecs + cluster - 1) / cluster;
+        int const partVecs = share < kPartVecs ? share : kPartVecs;
+        int64_t const most = sms * kCtasPerSm / cluster * cluster, ctas = args.rows * cluster;
+        e = launchDependentCluster(&optIn, logProbsKernel<T, kReadingWarps>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)),
+            dim3((kReadingWarps + 1) * 32), static_cast<size_t>(partVecs) * 16, stream, cluster, args, cluster, partVecs);
     }
     if (e != cudaSuccess)
         B200_FAIL(BERT_B200_CUDA_ERROR, "logProbsKernel: %s", cudaGetErrorString(e));

@@ -43,9 +43,10 @@ def _check(T, cuda, x, ids, top, view=None):
     return r
 
 
-# vocabularies around vectors and parts: one warp per row up to 1016 halves / 508 floats, eight warps up to 8184 / 4092, then parts of 32768 / 16384
+# vocabularies around vectors and parts: one warp per row up to 504 halves / 252 floats (4088 / 2044 of many rows),
+# then eight warps, beyond 32760 / 16380 with several parts
 @pytest.mark.parametrize("dtype", ["fp16", "fp32"])
-@pytest.mark.parametrize("vocab", [1, 2, 5, 8, 31, 100, 500, 508, 509, 1016, 1017, 1100, 4092, 4093, 8184, 8185, 16385, 30522, 32768, 32769, 50001, 120000])
+@pytest.mark.parametrize("vocab", [1, 2, 5, 8, 31, 100, 252, 253, 500, 504, 505, 1016, 1100, 4092, 4093, 8184, 8185, 16385, 30522, 32768, 32769, 50001, 120000])
 def test_log_probs(cuda, dtype, vocab):
     import tensorrt_b200 as T
 
@@ -57,7 +58,7 @@ def test_log_probs(cuda, dtype, vocab):
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "fp32"])
-@pytest.mark.parametrize("rows,vocab", [(700, 50), (650, 3000), (400, 30522), (310, 70001)])
+@pytest.mark.parametrize("rows,vocab", [(700, 50), (650, 3000), (1300, 4001), (400, 30522), (310, 70001)])
 def test_log_probs_many_rows(cuda, dtype, rows, vocab):
     """More rows than fit the GPU: one CTA per row, also where a row has several parts."""
     import tensorrt_b200 as T
