@@ -222,38 +222,29 @@ __device__ __forceinline__ QuantStep fcEpilogueMath(uint32_t const (&r)[W], floa
 
 // The same with a scale for the row and one for each column: act((acc * rowScale) * colScale + bias). The accumulator is rounded to FP32
 // once (exact up to 2^24), the product with the row's scale and the multiply-add once each: at most 3 half steps of FP32 before the
-// activation. `colScale`, `bias` (null for none): of the first column; `validCols` columns of them may be read.
+// activation. `colScale`, `bias` (null for none): of the first column, in shared memory, W of them. Pairs of columns per instruction: 3.1
+// instructions per FP16 value without GELU against 2.9 with one scale per tensor.
 template <typename Out, int W>
-__device__ __forceinline__ void fcRowwiseMath(
-    uint32_t const (&r)[W], float (&v)[W], float rowScale, float const* colScale, float const* bias, int32_t act, int validCols)
+__device__ __forceinline__ void fcRowwiseMath(uint32_t const (&r)[W], float (&v)[W], float rowScale, float const* colScale, float const* bias, int32_t act)
 {
+    uint64_t const rs = pack2(rowScale, rowScale);
 #pragma unroll
     for (int j = 0; j < W; j += 4)
     {
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-        if (j + 4 <= validCols)
+        ulonglong2 const s = *reinterpret_cast<ulonglong2 const*>(colScale + j);
+        uint64_t const a = mul2(pack2(static_cast<float>(static_cast<int32_t>(r[j])), static_cast<float>(static_cast<int32_t>(r[j + 1]))), rs);
+        uint64_t const b = mul2(pack2(static_cast<float>(static_cast<int32_t>(r[j + 2])), static_cast<float>(static_cast<int32_t>(r[j + 3]))), rs);
+        if (bias)
         {
-            float4 const t = *reinterpret_cast<float4 const*>(colScale + j);
-            s[0] = t.x, s[1] = t.y, s[2] = t.z, s[3] = t.w;
-            if (bias)
-            {
-                float4 const u = *reinterpret_cast<float4 const*>(bias + j);
-                b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w;
-            }
+            ulonglong2 const c = *reinterpret_cast<ulonglong2 const*>(bias + j);
+            unpack2(fma2(a, s.x, c.x), v[j], v[j + 1]);
+            unpack2(fma2(b, s.y, c.y), v[j + 2], v[j + 3]);
         }
         else
         {
-#pragma unroll
-            for (int i = 0; i < 3; ++i)
-                if (j + i < validCols)
-                {
-                    s[i] = colScale[j + i];
-                    b[i] = bias ? bias[j + i] : 0.f;
-                }
+            unpack2(mul2(a, s.x), v[j], v[j + 1]);
+            unpack2(mul2(b, s.y), v[j + 2], v[j + 3]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v[j + i] = fmaf(static_cast<float>(static_cast<int32_t>(r[j + i])) * rowScale, s[i], b[i]);
     }
     if (act == BERT_B200_ACT_GELU_ERF)
     {
@@ -596,7 +587,7 @@ __global__ void __launch_bounds__(FcTileSmem<BLOCK_M, BLOCK_N, kRowwise>::kThrea
                     float v[kChunk];
                     QuantStep q{};
                     if constexpr (kRowwise)
-                        fcRowwiseMath<Out, kChunk>(r, v, rowScale, sScale + c * kChunk, args.bias ? sBias + c * kChunk : nullptr, args.act, kChunk);
+                        fcRowwiseMath<Out, kChunk>(r, v, rowScale, sScale + c * kChunk, args.bias ? sBias + c * kChunk : nullptr, args.act);
                     else
                         q = fcEpilogueMath<kInt8, Out, kChunk>(r, v, args, args.bias ? sBias + c * kChunk : nullptr, kChunk);
                     // rows of the block, padded by 16 bytes against bank conflicts; every piece is 16 bytes
@@ -695,16 +686,20 @@ int32_t launchFcTile(FcProblem const& p, bool weightsReady, cudaStream_t stream)
 //   CTAs; its "accEmpty" barriers collect the epilogue arrivals of both CTAs. tcgen05.commit multicasts the
 //   "stage free" and "accumulator ready" arrivals to both CTAs.
 // ------------------------------------------------------------------------------------------------
-template <int BLOCK_N>
+template <int BLOCK_N, typename Out, bool kRowwise>
 struct FcPairSmem
 {
     static constexpr int kABytes = kBlockM * kRowBytes;            // this CTA's 128 rows of A
     static constexpr int kBBytes = (BLOCK_N / 2) * kRowBytes;      // this CTA's half of the Wt rows
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = BLOCK_N == 128 ? 8 : (BLOCK_N == 160 ? 7 : 6);
+    // Row-wise: two stages less leave room for the columns' scales and biases and for a second staging tile.
+    static constexpr int kStages = (BLOCK_N == 128 ? 8 : (BLOCK_N == 160 ? 7 : 6)) - (kRowwise ? 2 : 0);
     static constexpr int kOutOff = kStages * kStageBytes;          // epilogue staging: kOutWarpBytes per epilogue warp
-    static constexpr int kOutWarpBytes = 2048;                     // one FP16 or two INT8 [32 x 32] chunks
-    static constexpr int kBarrierOff = kOutOff + kEpilogueWarps * kOutWarpBytes;
+    static constexpr int kOutTileBytes = 32 * (sizeof(Out) == 1 ? 32 : 64); // [32 x 32], FP32: [32 x 16]
+    static constexpr int kOutTiles = kRowwise || sizeof(Out) == 1 ? 2 : 1;
+    static constexpr int kOutWarpBytes = kOutTiles * kOutTileBytes;
+    static constexpr int kColumnsOff = kOutOff + kEpilogueWarps * kOutWarpBytes; // scales and biases of each warp's two chunks
+    static constexpr int kBarrierOff = kColumnsOff + (kRowwise ? kEpilogueWarps * 512 : 0);
     static constexpr int kTotal = kBarrierOff + (2 * kStages + 4) * 8 + 16;
     static constexpr int kDynamic = kTotal + 1024;
     static_assert(kDynamic <= 232448, "shared memory budget of one CTA");
@@ -715,7 +710,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFcThreads, 1)
     fcTcgen05PairKernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
         const __grid_constant__ CUtensorMap mapC, FcArgs const args)
 {
-    using L = FcPairSmem<BLOCK_N>;
+    using L = FcPairSmem<BLOCK_N, Out, kRowwise>;
     constexpr bool kInt8 = sizeof(In) == 1;
     constexpr int kBlockK = kRowBytes / sizeof(In);
     constexpr int kUmmaKBytes = 32;
@@ -908,8 +903,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFcThreads, 1)
         int const part = (warp - 2) >> 2;
         constexpr int kChunks = BLOCK_N / 32;
         constexpr int kChunksPerWarp = (kChunks + kEpilogueWarps / 4 - 1) / (kEpilogueWarps / 4); // one less in some warps
-        constexpr int kChunkBytes = 32 * 32 * static_cast<int>(sizeof(Out));
-        constexpr int kBufs = sizeof(Out) == 1 ? 2 : 1; // staging tiles of this warp: two for INT8; for FP32 one holds half a chunk
+        constexpr int kBufs = L::kOutTiles; // staging tiles of this warp
         uint8_t* const stage0 = smem + L::kOutOff + (warp - 2) * L::kOutWarpBytes;
         int buf = 0;
         int acc = 0;
@@ -919,9 +913,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFcThreads, 1)
             int64_t const rowBase = (tile / nBlocks) * kPairM + static_cast<int64_t>(rank) * kBlockM + quad * 32;
             int64_t const n0 = (tile % nBlocks) * BLOCK_N;
             float rowScale = 0.f;
+            float* const columns = reinterpret_cast<float*>(smem + L::kColumnsOff + (warp - 2) * 512); // per chunk: scales, biases
             if constexpr (kRowwise)
+            {
                 if (rowBase + lane < args.M)
                     rowScale = __ldg(args.rowScale + rowBase + lane);
+                float scale[kChunksPerWarp], bias[kChunksPerWarp];
+#pragma unroll
+                for (int i = 0; i < kChunksPerWarp; ++i)
+                {
+                    int64_t const c = n0 + (part + i * (kEpilogueWarps / 4)) * 32 + lane;
+                    scale[i] = c < args.N ? __ldg(args.colScale + c) : 0.f;
+                    bias[i] = c < args.N && args.bias ? __ldg(args.bias + c) : 0.f;
+                }
+                __syncwarp(); // the tile before has been read
+#pragma unroll
+                for (int i = 0; i < kChunksPerWarp; ++i)
+                {
+                    columns[i * 64 + lane] = scale[i];
+                    columns[i * 64 + 32 + lane] = bias[i];
+                }
+                __syncwarp();
+            }
             if (!mbarWait(&accFull[acc], accPhase, abortFlag, kWaitAccFull))
                 break;
             tcFenceAfter();
@@ -950,10 +963,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFcThreads, 1)
                     float v[32];
                     QuantStep q{};
                     if constexpr (kRowwise)
-                        fcRowwiseMath<Out, 32>(r, v, rowScale, args.colScale + col, args.bias ? args.bias + col : nullptr, args.act, validCols);
+                        fcRowwiseMath<Out, 32>(r, v, rowScale, columns + i * 64, args.bias ? columns + i * 64 + 32 : nullptr, args.act);
                     else
                         q = fcEpilogueMath<kInt8, Out, 32>(r, v, args, args.bias ? args.bias + col : nullptr, validCols);
-                    uint8_t* const tileBuf = stage0 + buf * kChunkBytes;
                     constexpr int kStores = sizeof(Out) == 4 ? 2 : 1;
                     // The TMA unit clips at 16 bytes: columns beyond the last whole piece are stored by the threads, each its row's.
                     constexpr int kPer = 16 / static_cast<int>(sizeof(Out));
@@ -969,6 +981,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFcThreads, 1)
 #pragma unroll
                     for (int h = 0; h < kStores; ++h)
                     {
+                        uint8_t* const tileBuf = stage0 + buf * L::kOutTileBytes;
                         if (lane == 0)
                             bulkWaitGroupRead<kBufs - 1>(); // the store that last used this staging tile has read it
                         __syncwarp();
@@ -984,8 +997,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFcThreads, 1)
                             tmaStore2d(&mapC, tileBuf, static_cast<int32_t>(col) + 16 * h, static_cast<int32_t>(rowBase));
                             bulkCommitGroup();
                         }
+                        buf = buf + 1 == kBufs ? 0 : buf + 1;
                     }
-                    buf = buf + 1 == kBufs ? 0 : buf + 1;
                 }
             }
             acc ^= 1;
@@ -1020,7 +1033,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFcThreads, 1)
 template <typename In, int BLOCK_N, typename Out, bool kRowwise = false>
 int32_t launchFcPair(FcProblem const& p, cudaStream_t stream)
 {
-    using L = FcPairSmem<BLOCK_N>;
+    using L = FcPairSmem<BLOCK_N, Out, kRowwise>;
     constexpr int kBlockK = kRowBytes / sizeof(In);
     CUtensorMapDataType const dt = sizeof(In) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap mapA, mapB;

@@ -229,10 +229,10 @@ def fc_rowwise(a, a_scales, wt, wt_scales, bias=None, activation=ACT_NONE, out_d
     n = wt.shape[0]
     per = 16 // out_dtype.itemsize
     if out is None:
-        padded = (n + per - 1) // per * per
-        out = torch.empty((m, padded), dtype=out_dtype, device=a.device)
-        if padded != n:
-            out = out[:, :n]
+        if n % per == 0:
+            out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+        else:  # whole lines of 128 bytes: 640 x 30522 FP32 44 us with rows padded to 16 bytes, 36 us so
+            out = torch.empty((m, -(-n // (8 * per)) * 8 * per), dtype=out_dtype, device=a.device)[:, :n]
     elif out.dtype != out_dtype or tuple(out.shape) != (m, n):
         raise ValueError(f"out must be a {out_dtype} tensor of shape {(m, n)}")
     p = _lib.FcRowwiseParams(_TYPE_ID[out_dtype], activation, m, n, k, a.data_ptr(), _row_stride(a, "a", 16), _vector(a_scales, m, "a_scales"),
