@@ -265,6 +265,14 @@ __device__ __forceinline__ float maxNan(float a, float b)
     return v;
 }
 
+// max(|a|, |b|, |c|), NaN if one of them is.
+__device__ __forceinline__ float maxAbsNan(float a, float b, float c)
+{
+    float v;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+
 __device__ __forceinline__ float warpMaxNan(float v)
 {
     float m;

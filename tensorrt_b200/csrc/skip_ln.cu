@@ -5,7 +5,7 @@
 // Replaces the reference kernels skipln_vec / skipLayerNormKernel[Small] / skiplnDQQ
 // (plugin/skipLayerNormPlugin/skipLayerNormKernel.cu:43-217) and skiplnDQQ_vec3/4,
 // skipln_vec32_hface/mtron (plugin/skipLayerNormPlugin/skipLayerNormInt8InterleavedKernel{HFace,MTron}.cu).
-#include "row_quant.cuh"
+#include "common.cuh"
 
 #include <limits>
 
@@ -40,25 +40,6 @@ __device__ __forceinline__ float rowSum(float v, float (*slots)[WPR > 1 ? WPR : 
 #pragma unroll
     for (int w = 0; w < WPR; ++w)
         t += slot[w];
-    return t;
-}
-
-// The same for the maximum of the row (NaN if one of its values is NaN).
-template <int WPR>
-__device__ __forceinline__ float rowMaxNan(float v, float (*slots)[WPR > 1 ? WPR : 1], int rowInCta, int wInRow, int lane, int& turn)
-{
-    v = warpMaxNan(v);
-    if (WPR == 1)
-        return v;
-    float* const slot = slots[turn];
-    turn ^= 1;
-    if (lane == 0)
-        slot[wInRow] = v;
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + rowInCta), "n"(WPR * 32) : "memory");
-    float t = slot[0];
-#pragma unroll
-    for (int w = 1; w < WPR; ++w)
-        t = maxNan(t, slot[w]);
     return t;
 }
 
@@ -144,12 +125,10 @@ __device__ __forceinline__ void prefetchParams(int32_t ld, T const* beta, T cons
 // One row is shared by WPR warps; each lane owns CPL 16-byte chunks: chunk (i*WPR + wInRow)*32 + lane.
 // The grid strides over rows, so gamma/beta/bias chunks (always the same columns for a lane) stay
 // in L1 after the first row.
-// QUANT: the row is also quantised to INT8 with a scale of its own, from the FP32 results while they are in registers (one more
-// reduction; `skip` and `out` may be null then). What goes to `out` has the same bits either way.
-template <typename T, int CPL, int WPR, bool HAS_BIAS, bool QUANT>
+template <typename T, int CPL, int WPR, bool HAS_BIAS>
 __global__ void __launch_bounds__(kThreads, (WPR == 2 && CPL == 2) ? 4 : 1) skipLnKernel(int32_t const ld, int64_t const rows, T const* __restrict__ in,
     T const* __restrict__ skip, T const* __restrict__ beta, T const* __restrict__ gamma, T const* __restrict__ bias,
-    T* __restrict__ out, float const eps, int8_t* __restrict__ outI8, float* __restrict__ rowScales)
+    T* __restrict__ out, float const eps)
 {
     constexpr int E = Vec<T>::kElems;
     constexpr int kRowsPerCta = kWarpsPerCta / WPR;
@@ -178,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, (WPR == 2 && CPL == 2) ? 4 : 1) skip
             int const c = (i * WPR + wInRow) * 32 + lane;
             bool const ok = rOk && c < chunksPerRow;
             a[i] = ok ? ldgStream(in + r * ld + c * E) : make_uint4(0, 0, 0, 0);
-            b[i] = ok && (!QUANT || skip) ? ldgStream(skip + r * ld + c * E) : make_uint4(0, 0, 0, 0);
+            b[i] = ok ? ldgStream(skip + r * ld + c * E) : make_uint4(0, 0, 0, 0);
         }
     };
     // Rows shared by four or more warps (4096 values and up) load their next row while the statistics and the store of
@@ -239,7 +218,6 @@ __global__ void __launch_bounds__(kThreads, (WPR == 2 && CPL == 2) ? 4 : 1) skip
         float const var = rowSum<WPR>(q, red[rowInCta], rowInCta, wInRow, lane, turn) * rld;
         float const rsigma = rsqrtf(var + eps);
 
-        float most = 0.f;
 #pragma unroll
         for (int i = 0; i < CPL; ++i)
         {
@@ -252,44 +230,17 @@ __global__ void __launch_bounds__(kThreads, (WPR == 2 && CPL == 2) ? 4 : 1) skip
 #pragma unroll
                 for (int j = 0; j < E; ++j)
                     x[i][j] = g[j] * (x[i][j] - mu) * rsigma + bt[j];
-                if (!QUANT || out)
-                    stgStream(out + row * ld + c * E, Vec<T>::pack(x[i]));
-                if constexpr (QUANT)
-                {
-#pragma unroll
-                    for (int j = 0; j < E; ++j)
-                        most = maxNan(most, fabsf(x[i][j]));
-                }
-            }
-        }
-        if constexpr (QUANT)
-        {
-            RowScale const rs = makeRowScale(rowMaxNan<WPR>(most, red[rowInCta], rowInCta, wInRow, lane, turn));
-            if (rowOk && wInRow == 0 && lane == 0)
-                rowScales[row] = rs.scale;
-#pragma unroll
-            for (int i = 0; i < CPL; ++i)
-            {
-                int const c = (i * WPR + wInRow) * 32 + lane;
-                if (rowOk && c < chunksPerRow)
-                {
-                    uint32_t w[E / 4];
-                    quantRowChunk<E, true>(x[i], rs, w);
-                    if constexpr (E == 8)
-                        stgStream8(outI8 + row * ld + c * E, make_uint2(w[0], w[1]));
-                    else
-                        *reinterpret_cast<uint32_t*>(outI8 + row * ld + c * E) = w[0];
-                }
+                stgStream(out + row * ld + c * E, Vec<T>::pack(x[i]));
             }
         }
     }
 }
 
 // Any ld, scalar accesses, one warp per row; the row is revisited from L1/L2 instead of registers.
-template <typename T, bool HAS_BIAS, bool QUANT>
+template <typename T, bool HAS_BIAS>
 __global__ void __launch_bounds__(kThreads) skipLnScalarKernel(int32_t const ld, int64_t const rows,
     T const* __restrict__ in, T const* __restrict__ skip, T const* __restrict__ beta, T const* __restrict__ gamma,
-    T const* __restrict__ bias, T* __restrict__ out, float const eps, int8_t* __restrict__ outI8, float* __restrict__ rowScales)
+    T const* __restrict__ bias, T* __restrict__ out, float const eps)
 {
     int const lane = threadIdx.x & 31;
     int const warp = threadIdx.x >> 5;
@@ -299,43 +250,23 @@ __global__ void __launch_bounds__(kThreads) skipLnScalarKernel(int32_t const ld,
     {
         T const* a = in + row * ld;
         T const* b = skip + row * ld;
-        auto value = [&](int i) {
-            return static_cast<float>(a[i]) + (!QUANT || skip ? static_cast<float>(b[i]) : 0.f) + (HAS_BIAS ? static_cast<float>(bias[i]) : 0.f);
-        };
         float s = 0.f;
         for (int i = lane; i < ld; i += 32)
-            s += value(i);
+            s += static_cast<float>(a[i]) + static_cast<float>(b[i]) + (HAS_BIAS ? static_cast<float>(bias[i]) : 0.f);
         float const mu = warpSum(s) * rld;
         float q = 0.f;
         for (int i = lane; i < ld; i += 32)
         {
-            float const d = value(i) - mu;
+            float const d
+                = static_cast<float>(a[i]) + static_cast<float>(b[i]) + (HAS_BIAS ? static_cast<float>(bias[i]) : 0.f) - mu;
             q += d * d;
         }
         float const rsigma = rsqrtf(warpSum(q) * rld + eps);
-        auto result = [&](int i) {
-            return static_cast<float>(gamma[i]) * (value(i) - mu) * rsigma + static_cast<float>(beta[i]);
-        };
-        if constexpr (QUANT)
+        for (int i = lane; i < ld; i += 32)
         {
-            float most = 0.f;
-            for (int i = lane; i < ld; i += 32)
-                most = maxNan(most, fabsf(result(i)));
-            RowScale const rs = makeRowScale(warpMaxNan(most));
-            if (lane == 0)
-                rowScales[row] = rs.scale;
-            for (int i = lane; i < ld; i += 32)
-            {
-                float const y = result(i); // read before it is written, so that `out` may be the input's rows
-                outI8[row * ld + i] = quantRowValue<true>(y, rs);
-                if (out)
-                    out[row * ld + i] = static_cast<T>(y);
-            }
-        }
-        else
-        {
-            for (int i = lane; i < ld; i += 32)
-                out[row * ld + i] = static_cast<T>(result(i));
+            float const v
+                = static_cast<float>(a[i]) + static_cast<float>(b[i]) + (HAS_BIAS ? static_cast<float>(bias[i]) : 0.f);
+            out[row * ld + i] = static_cast<T>(static_cast<float>(gamma[i]) * (v - mu) * rsigma + static_cast<float>(beta[i]));
         }
     }
 }
@@ -1024,36 +955,38 @@ inline int gridFor(int64_t groups, int ctasPerSm)
     return static_cast<int>((groups + passes - 1) / passes);
 }
 
-template <typename T, int CPL, int WPR, bool QUANT>
+template <typename T, int CPL, int WPR>
 int32_t launchSkipLn(cudaStream_t stream, int32_t ld, int64_t rows, T const* in, T const* skip, T const* beta,
-    T const* gamma, T const* bias, T* out, float eps, int8_t* outI8, float* rowScales)
+    T const* gamma, T const* bias, T* out, float eps)
 {
     int const rowsPerCta = kWarpsPerCta / WPR;
     int const grid = gridFor((rows + rowsPerCta - 1) / rowsPerCta, 8);
     if (bias)
-        launchDependent(skipLnKernel<T, CPL, WPR, true, QUANT>, dim3(grid), dim3(kThreads), 0, stream, ld, rows, in, skip, beta, gamma, bias,
-            out, eps, outI8, rowScales);
+        launchDependent(skipLnKernel<T, CPL, WPR, true>, dim3(grid), dim3(kThreads), 0, stream, ld, rows, in, skip, beta, gamma, bias,
+            out, eps);
     else
-        launchDependent(skipLnKernel<T, CPL, WPR, false, QUANT>, dim3(grid), dim3(kThreads), 0, stream, ld, rows, in, skip, beta, gamma, bias,
-            out, eps, outI8, rowScales);
+        launchDependent(skipLnKernel<T, CPL, WPR, false>, dim3(grid), dim3(kThreads), 0, stream, ld, rows, in, skip, beta, gamma, bias,
+            out, eps);
     return checkLaunch("skipLnKernel");
 }
 
-// QUANT: `outI8` and `rowScales` receive the quantised rows.
-template <typename T, bool QUANT>
+template <typename T>
 int32_t dispatchSkipLn(cudaStream_t stream, int32_t ld, int64_t rows, T const* in, T const* skip, T const* beta,
-    T const* gamma, T const* bias, T* out, float eps, int8_t* outI8, float* rowScales)
+    T const* gamma, T const* bias, T* out)
 {
+    // FP16: the reference adds numeric_limits<half>::epsilon(), which is value-initialised (0) because no
+    // specialisation for __half exists; FP32 adds 1.19e-7 (plugin/skipLayerNormPlugin/skipLayerNormKernel.cu:149).
+    float const eps = sizeof(T) == 4 ? std::numeric_limits<float>::epsilon() : 0.f;
     constexpr int E = 16 / sizeof(T);
     bool const vec = (ld % E == 0) && ld / E <= 32 * 4 * 8 && aligned16(in) && aligned16(skip) && aligned16(out)
-        && aligned16(beta) && aligned16(gamma) && (!bias || aligned16(bias)) && reinterpret_cast<uintptr_t>(outI8) % E == 0;
+        && aligned16(beta) && aligned16(gamma) && (!bias || aligned16(bias));
     if (!vec)
     {
         int const grid = gridFor((rows + kWarpsPerCta - 1) / kWarpsPerCta, 8);
         if (bias)
-            skipLnScalarKernel<T, true, QUANT><<<grid, kThreads, 0, stream>>>(ld, rows, in, skip, beta, gamma, bias, out, eps, outI8, rowScales);
+            skipLnScalarKernel<T, true><<<grid, kThreads, 0, stream>>>(ld, rows, in, skip, beta, gamma, bias, out, eps);
         else
-            skipLnScalarKernel<T, false, QUANT><<<grid, kThreads, 0, stream>>>(ld, rows, in, skip, beta, gamma, bias, out, eps, outI8, rowScales);
+            skipLnScalarKernel<T, false><<<grid, kThreads, 0, stream>>>(ld, rows, in, skip, beta, gamma, bias, out, eps);
         return checkLaunch("skipLnScalarKernel");
     }
     int const chunks = ld / E;
@@ -1068,7 +1001,7 @@ int32_t dispatchSkipLn(cudaStream_t stream, int32_t ld, int64_t rows, T const* i
     int const cpl = (chunks + 32 * wpr - 1) / (32 * wpr);
 #define B200_SKIPLN_CASE(C, W)                                                                                         \
     if (cpl == C && wpr == W)                                                                                          \
-        return launchSkipLn<T, C, W, QUANT>(stream, ld, rows, in, skip, beta, gamma, bias, out, eps, outI8, rowScales);
+        return launchSkipLn<T, C, W>(stream, ld, rows, in, skip, beta, gamma, bias, out, eps);
     B200_SKIPLN_CASE(1, 1)
     B200_SKIPLN_CASE(2, 1)
     B200_SKIPLN_CASE(3, 1)
@@ -1189,36 +1122,15 @@ extern "C" int32_t bert_b200_skip_layer_norm(void* stream, int32_t type_id, int3
         return BERT_B200_OK;
     B200_REQUIRE(input && skip && beta && gamma && output, "skip_layer_norm: null pointer");
     auto s = static_cast<cudaStream_t>(stream);
-    // FP16: the reference adds numeric_limits<half>::epsilon(), which is value-initialised (0) because no
-    // specialisation for __half exists; FP32 adds 1.19e-7 (plugin/skipLayerNormPlugin/skipLayerNormKernel.cu:149).
     if (type_id == BERT_B200_FP16)
-        return dispatchSkipLn<__half, false>(s, ld, n / ld, static_cast<__half const*>(input), static_cast<__half const*>(skip),
+        return dispatchSkipLn<__half>(s, ld, n / ld, static_cast<__half const*>(input), static_cast<__half const*>(skip),
             static_cast<__half const*>(beta), static_cast<__half const*>(gamma), static_cast<__half const*>(bias),
-            static_cast<__half*>(output), 0.f, nullptr, nullptr);
+            static_cast<__half*>(output));
     if (type_id == BERT_B200_FP32)
-        return dispatchSkipLn<float, false>(s, ld, n / ld, static_cast<float const*>(input), static_cast<float const*>(skip),
+        return dispatchSkipLn<float>(s, ld, n / ld, static_cast<float const*>(input), static_cast<float const*>(skip),
             static_cast<float const*>(beta), static_cast<float const*>(gamma), static_cast<float const*>(bias),
-            static_cast<float*>(output), std::numeric_limits<float>::epsilon(), nullptr, nullptr);
+            static_cast<float*>(output));
     B200_FAIL(BERT_B200_NOT_SUPPORTED, "skip_layer_norm: type_id %d (INT8 uses bert_b200_skip_layer_norm_dqq)", type_id);
-}
-
-extern "C" int32_t bert_b200_skip_layer_norm_quantize(void* stream, int32_t type_id, int32_t ld, int64_t n, void const* input, void const* skip,
-    void const* beta, void const* gamma, void* output, int8_t* out_i8, float* row_scales, void const* bias, float eps)
-{
-    B200_REQUIRE(type_id == BERT_B200_FP16 || type_id == BERT_B200_FP32, "skip_layer_norm_quantize: type_id %d (FP16 or FP32)", type_id);
-    B200_REQUIRE(ld > 0 && n >= 0 && n % ld == 0, "skip_layer_norm_quantize: n=%lld is not a multiple of ld=%d", static_cast<long long>(n), ld);
-    B200_REQUIRE(eps >= 0.f, "skip_layer_norm_quantize: eps must not be negative");
-    if (n == 0)
-        return BERT_B200_OK;
-    B200_REQUIRE(input && beta && gamma && out_i8 && row_scales, "skip_layer_norm_quantize: null pointer");
-    auto s = static_cast<cudaStream_t>(stream);
-    if (type_id == BERT_B200_FP16)
-        return dispatchSkipLn<__half, true>(s, ld, n / ld, static_cast<__half const*>(input), static_cast<__half const*>(skip),
-            static_cast<__half const*>(beta), static_cast<__half const*>(gamma), static_cast<__half const*>(bias), static_cast<__half*>(output), eps,
-            out_i8, row_scales);
-    return dispatchSkipLn<float, true>(s, ld, n / ld, static_cast<float const*>(input), static_cast<float const*>(skip),
-        static_cast<float const*>(beta), static_cast<float const*>(gamma), static_cast<float const*>(bias), static_cast<float*>(output), eps, out_i8,
-        row_scales);
 }
 
 // `paramsReady`: beta, gamma and bias were complete before the kernel ahead in the stream began, and so before those that it may
