@@ -483,6 +483,25 @@ typedef struct bert_b200_encoder bert_b200_encoder;
 BERT_B200_API int64_t bert_b200_encoder_workspace_size(bert_b200_encoder_config const* cfg, int32_t max_tokens,
     int32_t max_batch);
 BERT_B200_API int32_t bert_b200_encoder_create(bert_b200_encoder_config const* cfg, bert_b200_encoder** out);
+
+/*
+ * INT8 without calibration: the projections of `cfg` (type_id INT8) have INT8 weights [out][in] with a scale for each output channel
+ * (device vectors, here; bert_b200_quantize_rows makes both out of FP16 weights), their inputs are quantised row by row (token by token) on the way,
+ * and everything between them stays FP16 (attention, LayerNorm, GELU). The steps s_* of the layers and dq_probs are not used. All forward
+ * functions take such an encoder; its workspace is that of bert_b200_encoder_rowwise_workspace_size (calibration needs the FP16 encoder).
+ */
+typedef struct bert_b200_rowwise_scales
+{
+    float const* wt_qkv;  /* [3E] */
+    float const* wt_out;  /* [E] */
+    float const* wt_ffn1; /* [F] */
+    float const* wt_ffn2; /* [E] */
+} bert_b200_rowwise_scales;
+
+BERT_B200_API int64_t bert_b200_encoder_rowwise_workspace_size(bert_b200_encoder_config const* cfg, int32_t max_tokens,
+    int32_t max_batch);
+BERT_B200_API int32_t bert_b200_encoder_create_rowwise(bert_b200_encoder_config const* cfg,
+    bert_b200_rowwise_scales const* scales_host, bert_b200_encoder** out);
 BERT_B200_API int32_t bert_b200_encoder_destroy(bert_b200_encoder* enc);
 /* Number of kernels the last forward launched (for accounting). */
 BERT_B200_API int32_t bert_b200_encoder_last_launch_count(bert_b200_encoder const* enc);

@@ -70,3 +70,25 @@ def token_log_probs(logits, ids, top_k):
         tid[r, :len(best)] = best
         tlp[r, :len(best)] = d[best] - lse
     return lp, ent, tid, tlp, mean
+
+
+def encoder(p, ids, seg, cu, S):
+    """The encoder with row-wise INT8 projections in 64 bits, every stored tensor rounded to FP16: weights with a scale per output channel, each
+    projection's input with a scale per token (of the LayerNorm's unrounded result where a LayerNorm precedes it)."""
+    from oracle import bert_oracle as O
+
+    h = lambda t: t.astype(np.float16).astype(np.float64)
+    B = len(cu) - 1
+    x, _ = O.emb_layer_norm_var_seqlen(ids, seg, cu, p.word_emb, p.pos_emb, p.tok_emb, p.emb_gamma, p.emb_beta)
+    x = h(x)
+    q = quantize_rows(x)
+    for lp in p.layers:
+        weights = {n: quantize_rows(np.asarray(getattr(lp, n), np.float32).T) for n in ("w_qkv", "w_out", "w_ffn1", "w_ffn2")}
+        product = lambda a, name, bias=None, act=0: h(fc_rowwise(a[0], a[1], *weights[name], bias, act)[1])
+        ctx = h(O.mha(product(q, "w_qkv", lp.b_qkv), B, S, p.heads, x.shape[1] // p.heads, cu=cu))
+        y = layer_norm(product(quantize_rows(ctx), "w_out"), x, lp.ln1_gamma, lp.ln1_beta, lp.b_out, 0.0)
+        h1 = h(y)
+        f1 = product(quantize_rows(y), "w_ffn1", lp.b_ffn1, 1)
+        y = layer_norm(product(quantize_rows(f1), "w_ffn2"), h1, lp.ln2_gamma, lp.ln2_beta, lp.b_ffn2, 0.0)
+        x, q = h(y), quantize_rows(y)
+    return x

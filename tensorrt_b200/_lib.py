@@ -62,6 +62,10 @@ class LayerWeights(C.Structure):
                 ("s_ln1", f32), ("s_wffn1", f32), ("s_ffn1", f32), ("s_wffn2", f32), ("s_ffn2", f32), ("s_out", f32)]
 
 
+class RowwiseScales(C.Structure):
+    _fields_ = [("wt_qkv", vp), ("wt_out", vp), ("wt_ffn1", vp), ("wt_ffn2", vp)]
+
+
 class EncoderConfig(C.Structure):
     _fields_ = [("type_id", i32), ("num_layers", i32), ("hidden_size", i32), ("num_heads", i32), ("ffn_size", i32),
                 ("vocab_size", i32), ("max_positions", i32), ("type_vocab_size", i32), ("dq_probs", f32),
@@ -97,6 +101,8 @@ SIGNATURES = {
     "bert_b200_probe_mma_rate": (i32, [vp, i32, i32, vp, C.POINTER(f32)]),
     "bert_b200_encoder_workspace_size": (i64, [C.POINTER(EncoderConfig), i32, i32]),
     "bert_b200_encoder_create": (i32, [C.POINTER(EncoderConfig), C.POINTER(vp)]),
+    "bert_b200_encoder_rowwise_workspace_size": (i64, [C.POINTER(EncoderConfig), i32, i32]),
+    "bert_b200_encoder_create_rowwise": (i32, [C.POINTER(EncoderConfig), C.POINTER(RowwiseScales), C.POINTER(vp)]),
     "bert_b200_encoder_destroy": (i32, [vp]),
     "bert_b200_encoder_last_launch_count": (i32, [vp]),
     "bert_b200_encoder_enable_timing": (i32, [vp, i32]),

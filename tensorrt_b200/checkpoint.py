@@ -125,3 +125,57 @@ class PoolerHead:
             raise ValueError("PoolerHead: every sequence needs at least one token (its first row is the [CLS] row)")
         first = hidden.index_select(0, starts).contiguous()
         return torch.tanh(ops.fc(first, self.wt, bias=self.bias).float()).half()
+
+
+class MaskedLmHead:
+    """The head of `BertForMaskedLM` (`cls.predictions`: dense + erf-GELU + LayerNorm, then the product with the vocabulary) on top of the
+    encoder output, and what it is asked: log probabilities of given tokens, entropy, the most likely tokens. The product with the vocabulary is
+    usually tied to the word embeddings (no `decoder.weight` in the state dict). rowwise=True: both products in INT8 with a scale per token and per
+    output channel, logits FP32; False: FP16."""
+
+    def __init__(self, state_dict, device="cuda:0", rowwise=True, eps=1e-12):
+        import torch
+
+        from . import ops
+
+        p = "cls.predictions."
+        get = lambda *names: next(torch.from_numpy(_np(state_dict[n])) for n in names if n in state_dict).to(device)
+        dense = get(p + "transform.dense.weight")
+        decoder = get(p + "decoder.weight", "bert.embeddings.word_embeddings.weight", "embeddings.word_embeddings.weight")
+        self.vocab = decoder.shape[0]
+        self.rowwise, self.eps = rowwise, eps
+        self.dense_bias = get(p + "transform.dense.bias")
+        self.gamma, self.beta = (get(p + "transform.LayerNorm." + n).half() for n in ("weight", "bias"))
+        bias = get(p + "decoder.bias", p + "bias")  # where both are there, the product's own is the one that is added
+        if rowwise:
+            with torch.cuda.device(dense.device):
+                self.dense, self.dense_scales = ops.quantize_rows(dense)
+                self.decoder, self.decoder_scales = ops.quantize_rows(decoder)
+            self.bias = bias
+        else:  # the FP16 product takes whole 16 columns: rows of zeros behind the vocabulary
+            pad = -self.vocab % 16
+            self.dense = dense.half()
+            self.decoder = torch.nn.functional.pad(decoder, (0, 0, 0, pad)).half()
+            self.bias = torch.nn.functional.pad(bias, (0, pad))
+
+    def logits(self, hidden):
+        """hidden: FP16 [tokens, hidden] -> [tokens, vocab], FP32 (rowwise) or FP16."""
+        from . import ops
+
+        if self.rowwise:
+            q, s = ops.quantize_rows(hidden)
+            t = ops.fc_rowwise(q, s, self.dense, self.dense_scales, self.dense_bias, ops.ACT_GELU_ERF)
+            _, q, s = ops.skip_layer_norm_quantize(t, None, self.gamma, self.beta, eps=self.eps, with_output=False)
+            return ops.fc_rowwise(q, s, self.decoder, self.decoder_scales, self.bias, out_dtype=self.bias.dtype)
+        t = ops.fc(hidden, self.dense, self.dense_bias, ops.ACT_GELU_ERF)
+        y, _, _ = ops.skip_layer_norm_quantize(t, None, self.gamma, self.beta, eps=self.eps)
+        return ops.fc(y, self.decoder, self.bias)[:, :self.vocab]
+
+    def __call__(self, hidden, positions=None, token_ids=None, top_k=5):
+        """hidden: FP16 [total, hidden] (packed tokens); positions: the rows that are asked about (None: all); token_ids: int32 [positions, tokens] or
+        [positions] -> ops.LogProbs."""
+        from . import ops
+
+        if positions is not None:
+            hidden = hidden.index_select(0, positions)
+        return ops.token_log_probs(self.logits(hidden.contiguous()), token_ids, top_k)

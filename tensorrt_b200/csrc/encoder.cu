@@ -18,6 +18,9 @@ struct bert_b200_encoder
 {
     bert_b200_encoder_config cfg;
     std::vector<bert_b200_layer_weights> layers;
+    // INT8 with a scale per token and output channel instead of calibrated steps: the weights' scales, one per layer
+    bool rowwise = false;
+    std::vector<bert_b200_rowwise_scales> scales;
     int32_t lastLaunches = 0;
     // optional per-launch timing: events[2*i], events[2*i+1] bracket launch i of kind kinds[i]
     bool timing = false;
@@ -49,6 +52,7 @@ namespace b200
 {
 
 int32_t fcRun(bert_b200_fc_params const& p, cudaStream_t stream, bool weightsReady);
+int32_t fcRowwiseRun(bert_b200_fc_rowwise_params const& p, cudaStream_t stream, bool weightsReady);
 int32_t skipLnDqqRun(cudaStream_t s, int32_t ld, int64_t n, int8_t const* input, int8_t const* skip, void const* beta, void const* gamma,
     int8_t* output, void const* bias, float dq_scale_in, float dq_scale_skip, float q_scale, bool paramsReady);
 
@@ -73,12 +77,15 @@ struct Workspace
     uint8_t* h1;   // [T][E]
     uint8_t* f1;   // [T][F]
     uint8_t* xf16; // [T][E]   FP16 copy of the embedding output (INT8 mode)
+    int8_t* q;     // [T][max(E, F)] the quantised input of the next layer (row-wise mode), then its scales [T]
+    float* scales;
     int64_t bytes;
 };
 
-Workspace carve(bert_b200_encoder_config const& c, int32_t maxTokens, int32_t maxBatch, void* base)
+Workspace carve(bert_b200_encoder_config const& c, bool rowwise, int32_t maxTokens, int32_t maxBatch, void* base)
 {
-    int64_t const elem = c.type_id == BERT_B200_INT8 ? 1 : 2;
+    bool const i8 = c.type_id == BERT_B200_INT8 && !rowwise; // row-wise: FP16 between the layers
+    int64_t const elem = i8 ? 1 : 2;
     int64_t const T = maxTokens;
     int64_t const E = c.hidden_size;
     int64_t const F = c.ffn_size;
@@ -98,7 +105,9 @@ Workspace carve(bert_b200_encoder_config const& c, int32_t maxTokens, int32_t ma
     int64_t const oAo = take(T * E * elem);
     int64_t const oH1 = take(T * E * elem);
     int64_t const oF1 = take(T * F * elem);
-    int64_t const oXf = c.type_id == BERT_B200_INT8 ? take(T * E * 2) : oX;
+    int64_t const oXf = i8 ? take(T * E * 2) : oX;
+    int64_t const oQ = rowwise ? take(T * (E > F ? E : F)) : oX;
+    int64_t const oScales = rowwise ? take(T * 4) : oX;
     Workspace w{};
     auto* b = static_cast<uint8_t*>(base);
     w.ids = reinterpret_cast<int32_t*>(b + oIds);
@@ -112,6 +121,8 @@ Workspace carve(bert_b200_encoder_config const& c, int32_t maxTokens, int32_t ma
     w.h1 = b + oH1;
     w.f1 = b + oF1;
     w.xf16 = b + oXf;
+    w.q = reinterpret_cast<int8_t*>(b + oQ);
+    w.scales = reinterpret_cast<float*>(b + oScales);
     w.bytes = off;
     return w;
 }
@@ -187,10 +198,17 @@ extern "C" int64_t bert_b200_encoder_workspace_size(bert_b200_encoder_config con
 {
     if (checkConfig(cfg) != BERT_B200_OK || max_tokens < 0 || max_batch < 0)
         return -1;
-    return carve(*cfg, max_tokens, max_batch, nullptr).bytes;
+    return carve(*cfg, false, max_tokens, max_batch, nullptr).bytes;
 }
 
-extern "C" int32_t bert_b200_encoder_create(bert_b200_encoder_config const* cfg, bert_b200_encoder** out)
+extern "C" int64_t bert_b200_encoder_rowwise_workspace_size(bert_b200_encoder_config const* cfg, int32_t max_tokens, int32_t max_batch)
+{
+    if (checkConfig(cfg) != BERT_B200_OK || cfg->type_id != BERT_B200_INT8 || max_tokens < 0 || max_batch < 0)
+        return -1;
+    return carve(*cfg, true, max_tokens, max_batch, nullptr).bytes;
+}
+
+static int32_t createEncoder(bert_b200_encoder_config const* cfg, bert_b200_rowwise_scales const* scales, bert_b200_encoder** out)
 {
     int32_t const st = checkConfig(cfg);
     if (st != BERT_B200_OK)
@@ -211,7 +229,18 @@ extern "C" int32_t bert_b200_encoder_create(bert_b200_encoder_config const* cfg,
             B200_FAIL(BERT_B200_BAD_PARAM, "encoder_create: null layer weight pointer");
         }
     }
-    if (cfg->type_id == BERT_B200_INT8)
+    if (scales)
+    {
+        e->rowwise = true;
+        e->scales.assign(scales, scales + cfg->num_layers);
+        for (auto const& s : e->scales)
+            if (!(s.wt_qkv && s.wt_out && s.wt_ffn1 && s.wt_ffn2))
+            {
+                delete e;
+                B200_FAIL(BERT_B200_BAD_PARAM, "encoder_create_rowwise: null pointer to a weight's scales");
+            }
+    }
+    else if (cfg->type_id == BERT_B200_INT8)
     {
         // a zero or non-finite scale turns 1 / s into inf / NaN inside the quantising epilogues, and a layer that
         // dequantises its input with another step than the one the previous layer quantised with is silently wrong
@@ -237,6 +266,19 @@ extern "C" int32_t bert_b200_encoder_create(bert_b200_encoder_config const* cfg,
     return BERT_B200_OK;
 }
 
+extern "C" int32_t bert_b200_encoder_create(bert_b200_encoder_config const* cfg, bert_b200_encoder** out)
+{
+    return createEncoder(cfg, nullptr, out);
+}
+
+extern "C" int32_t bert_b200_encoder_create_rowwise(
+    bert_b200_encoder_config const* cfg, bert_b200_rowwise_scales const* scales_host, bert_b200_encoder** out)
+{
+    B200_REQUIRE(cfg && cfg->type_id == BERT_B200_INT8, "encoder_create_rowwise: needs an INT8 configuration");
+    B200_REQUIRE(scales_host != nullptr, "encoder_create_rowwise: null scales");
+    return createEncoder(cfg, scales_host, out);
+}
+
 extern "C" int32_t bert_b200_encoder_destroy(bert_b200_encoder* enc)
 {
     delete enc;
@@ -252,7 +294,8 @@ static int32_t forwardImpl(bert_b200_encoder* enc, cudaStream_t stream, int32_t 
     int32_t const* ids, int32_t const* seg, int32_t const* cu, Workspace const& w, void* output)
 {
     bert_b200_encoder_config const& c = enc->cfg;
-    bool const i8 = c.type_id == BERT_B200_INT8;
+    bool const rowwise = enc->rowwise;
+    bool const i8 = c.type_id == BERT_B200_INT8 && !rowwise;
     int32_t const E = c.hidden_size;
     int32_t const F = c.ffn_size;
     int64_t const T = total;
@@ -315,6 +358,70 @@ static int32_t forwardImpl(bert_b200_encoder* enc, cudaStream_t stream, int32_t 
 
     int32_t const headSize = c.hidden_size / c.num_heads;
     float const rsqrtD = 1.f / std::sqrt(static_cast<float>(headSize));
+    if (rowwise)
+    {
+        // FP16 between the layers; what a projection multiplies is quantised row by row, by the LayerNorm that writes it or, behind attention and
+        // GELU, by a kernel of its own. w.q and w.scales always hold the next projection's input.
+        auto quantize = [&](void const* x, int32_t width) {
+            return bert_b200_quantize_rows(stream, BERT_B200_FP16, T, width, x, width, w.q, width, w.scales);
+        };
+        B200_STEP(BERT_B200_KIND_OTHER, quantize(w.x, E));
+        for (int32_t li = 0; li < c.num_layers; ++li)
+        {
+            bert_b200_layer_weights const& l = enc->layers[li];
+            bert_b200_rowwise_scales const& s = enc->scales[li];
+            auto project = [&](int32_t n, int32_t k, void const* wt, float const* wtScales, void* to, float const* bias, int32_t activation) {
+                bert_b200_fc_rowwise_params fc{};
+                fc.out_type_id = BERT_B200_FP16;
+                fc.activation = activation;
+                fc.m = T;
+                fc.n = n;
+                fc.k = k;
+                fc.a = w.q;
+                fc.lda = k;
+                fc.a_scales = w.scales;
+                fc.wt = static_cast<int8_t const*>(wt);
+                fc.ldw = k;
+                fc.wt_scales = wtScales;
+                fc.c = to;
+                fc.ldc = n;
+                fc.bias = bias;
+                fc.status_word = w.status;
+                return fcRowwiseRun(fc, stream, true);
+            };
+            B200_STEP(BERT_B200_KIND_FC, project(3 * E, E, l.wt_qkv, s.wt_qkv, w.qkv, l.b_qkv, BERT_B200_ACT_NONE));
+            bert_b200_mha_params mha{};
+            mha.type_id = BERT_B200_FP16;
+            mha.B = B;
+            mha.S = maxSeqlen;
+            mha.num_heads = c.num_heads;
+            mha.head_size = headSize;
+            mha.total = total;
+            mha.qkv = w.qkv;
+            mha.out = w.ctx;
+            mha.cu_seqlens = cu;
+            mha.scale_bmm1 = rsqrtD;
+            mha.scale_softmax = 1.f;
+            mha.scale_bmm2 = 1.f;
+            mha.status_word = w.status;
+            B200_STEP(BERT_B200_KIND_MHA, bert_b200_mha(&mha, stream));
+            B200_STEP(BERT_B200_KIND_OTHER, quantize(w.ctx, E));
+            B200_STEP(BERT_B200_KIND_FC, project(E, E, l.wt_out, s.wt_out, w.ao, nullptr, BERT_B200_ACT_NONE));
+            B200_STEP(BERT_B200_KIND_SKIPLN, bert_b200_skip_layer_norm_quantize(stream, BERT_B200_FP16, E, T * E, w.ao, w.x, l.ln1_beta, l.ln1_gamma,
+                w.h1, w.q, w.scales, l.b_out, 0.f));
+            B200_STEP(BERT_B200_KIND_FC, project(F, E, l.wt_ffn1, s.wt_ffn1, w.f1, l.b_ffn1, BERT_B200_ACT_GELU_ERF));
+            B200_STEP(BERT_B200_KIND_OTHER, quantize(w.f1, F));
+            B200_STEP(BERT_B200_KIND_FC, project(E, F, l.wt_ffn2, s.wt_ffn2, w.ao, nullptr, BERT_B200_ACT_NONE));
+            if (li + 1 == c.num_layers)
+                B200_STEP(BERT_B200_KIND_SKIPLN,
+                    bert_b200_skip_layer_norm(stream, BERT_B200_FP16, E, T * E, w.ao, w.h1, l.ln2_beta, l.ln2_gamma, output, l.b_ffn2));
+            else
+                B200_STEP(BERT_B200_KIND_SKIPLN, bert_b200_skip_layer_norm_quantize(stream, BERT_B200_FP16, E, T * E, w.ao, w.h1, l.ln2_beta,
+                    l.ln2_gamma, w.x, w.q, w.scales, l.b_ffn2, 0.f));
+        }
+        enc->lastLaunches = launches;
+        return BERT_B200_OK;
+    }
     for (int32_t li = 0; li < c.num_layers; ++li)
     {
         bert_b200_layer_weights const& l = enc->layers[li];
@@ -447,7 +554,7 @@ static int32_t checkForward(bert_b200_encoder* enc, int32_t B, int32_t total, in
         maxSeqlen, enc->cfg.max_positions);
     B200_REQUIRE(a && b && c && workspace && output, "encoder_forward: null pointer");
     B200_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 1023u) == 0, "encoder_forward: workspace must be 1024-byte aligned");
-    *w = carve(enc->cfg, total, B, workspace);
+    *w = carve(enc->cfg, enc->rowwise, total, B, workspace);
     B200_REQUIRE(w->bytes <= workspaceBytes, "encoder_forward: workspace too small (%lld < %lld)",
         static_cast<long long>(workspaceBytes), static_cast<long long>(w->bytes));
     return BERT_B200_OK;
@@ -662,7 +769,7 @@ extern "C" int32_t bert_b200_encoder_forward_static(bert_b200_encoder* enc, void
     B200_REQUIRE(enc != nullptr, "encoder_forward_static: null encoder");
     B200_REQUIRE(!enc->timing, "encoder_forward_static: per-kernel timing creates CUDA events; disable it for this entry point");
     B200_REQUIRE(B > 0 && total > 0, "encoder_forward_static: bad sizes B=%d total=%d", B, total);
-    int64_t const need = carve(enc->cfg, total, B, nullptr).bytes;
+    int64_t const need = carve(enc->cfg, enc->rowwise, total, B, nullptr).bytes;
     if (need > kStaticWorkspaceBytes)
         B200_FAIL(BERT_B200_NOT_SUPPORTED,
             "encoder_forward_static: %d tokens / %d sequences need %lld bytes of scratch, the built-in buffer holds %lld; "

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .ops import FP16, INT8
+from .ops import FP16, INT8, quantize_rows
 
 
 def _dev(a, dtype, device, transpose=False):
@@ -29,11 +29,16 @@ class BertEncoder:
     emb_beta, dq_probs and layers[i].{w_qkv [E,3E], b_qkv, w_out, b_out, ln1_gamma, ln1_beta, w_ffn1, b_ffn1,
     w_ffn2, b_ffn2, ln2_gamma, ln2_beta, scales}. FC weights arrive as [in, out] (the reference FC plugin's `W`
     field, plugin/fcPlugin/README.md:45) and are stored transposed [out, in] for the K-major tensor-core tiles.
-    For type_id INT8, layers[i].scales holds q_w_* (INT8 weights) and the s_* dequantisation steps."""
+    For type_id INT8, layers[i].scales holds q_w_* (INT8 weights) and the s_* dequantisation steps. With rowwise=True INT8 needs no
+    calibration and no scales: the floating-point weights are quantised here, a scale per output channel, and every projection's input on the
+    way, a scale per token; attention, LayerNorm and GELU stay FP16."""
 
-    def __init__(self, params, type_id=FP16, device="cuda:0"):
+    def __init__(self, params, type_id=FP16, device="cuda:0", rowwise=False):
+        if rowwise and type_id != INT8:
+            raise ValueError("rowwise scales go with type_id INT8")
         self.device = torch.device(device)
         self.type_id = type_id
+        self.rowwise = rowwise
         self.hidden = params.hidden
         self.heads = params.heads
         self.ffn = params.ffn
@@ -51,9 +56,16 @@ class BertEncoder:
         self.emb_beta = _dev(params.emb_beta, torch.float32, d)
         n_layers = len(params.layers)
         self._layers = (_lib.LayerWeights * n_layers)()
+        self._scales = (_lib.RowwiseScales * n_layers)()
         for i, lp in enumerate(params.layers):
             lw = self._layers[i]
-            if type_id == INT8:
+            if rowwise:
+                with torch.cuda.device(d):
+                    for name in ("qkv", "out", "ffn1", "ffn2"):
+                        q, s = quantize_rows(_dev(getattr(lp, "w_" + name), torch.float32, d, transpose=True))
+                        setattr(lw, "wt_" + name, keep(q))
+                        setattr(self._scales[i], "wt_" + name, keep(s))
+            elif type_id == INT8:
                 s = lp.scales
                 wq = lambda name: keep(_dev(s["q_" + name], torch.int8, d, transpose=True))
                 lw.wt_qkv, lw.wt_out, lw.wt_ffn1, lw.wt_ffn2 = wq("w_qkv"), wq("w_out"), wq("w_ffn1"), wq("w_ffn2")
@@ -74,7 +86,10 @@ class BertEncoder:
             C.c_void_p(self.pos_emb.data_ptr()), C.c_void_p(self.tok_emb.data_ptr()),
             C.c_void_p(self.emb_gamma.data_ptr()), C.c_void_p(self.emb_beta.data_ptr()), self._layers)
         handle = C.c_void_p()
-        check(lib.bert_b200_encoder_create(C.byref(self.cfg), C.byref(handle)), "encoder_create")
+        if rowwise:
+            check(lib.bert_b200_encoder_create_rowwise(C.byref(self.cfg), self._scales, C.byref(handle)), "encoder_create_rowwise")
+        else:
+            check(lib.bert_b200_encoder_create(C.byref(self.cfg), C.byref(handle)), "encoder_create")
         self._h = handle
         self._ws = None
         self._ws_key = (0, 0)
@@ -90,7 +105,8 @@ class BertEncoder:
     def _workspace(self, total, B):
         if self._ws is None or total > self._ws_key[0] or B > self._ws_key[1]:
             t, b = max(total, self._ws_key[0]), max(B, self._ws_key[1])
-            n = lib.bert_b200_encoder_workspace_size(C.byref(self.cfg), t, b)
+            size = lib.bert_b200_encoder_rowwise_workspace_size if self.rowwise else lib.bert_b200_encoder_workspace_size
+            n = size(C.byref(self.cfg), t, b)
             if n < 0:
                 raise RuntimeError("encoder_workspace_size failed")
             # torch's caching allocator returns 512-byte aligned blocks; over-allocate and align to 1024

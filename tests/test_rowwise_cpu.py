@@ -97,3 +97,31 @@ def test_oracle_of_quantised_rows():
         most = max(abs(Fraction(float(v))) for v in x[r])
         for j in range(30):
             assert q[r, j] == round(127 * Fraction(float(x[r, j])) / most)  # halves to even
+
+
+def test_rowwise_encoder_refusals():
+    L = _lib()
+    layers = (L.LayerWeights * 2)()
+    scales = (L.RowwiseScales * 2)()
+    for lw in layers:
+        for n, _ in L.LayerWeights._fields_:
+            if not n.startswith("s_"):
+                setattr(lw, n, C.c_void_p(FAKE))
+    for s in scales:
+        for n, _ in L.RowwiseScales._fields_:
+            setattr(s, n, C.c_void_p(FAKE))
+    f = C.c_void_p(FAKE)
+    make = lambda type_id: L.EncoderConfig(type_id, 2, 128, 2, 512, 100, 64, 2, 0.0, f, f, f, f, f, layers)
+    h = C.c_void_p()
+    cfg = make(2)
+    assert L.lib.bert_b200_encoder_create_rowwise(C.byref(cfg), scales, C.byref(h)) == 0     # no steps, no dq_probs needed
+    L.lib.bert_b200_encoder_destroy(h)
+    plain, rowwise = (f(C.byref(cfg), 100, 4) for f in (L.lib.bert_b200_encoder_workspace_size, L.lib.bert_b200_encoder_rowwise_workspace_size))
+    assert rowwise > plain > 0
+    assert L.lib.bert_b200_encoder_rowwise_workspace_size(C.byref(make(1)), 100, 4) == -1
+    assert L.lib.bert_b200_encoder_create_rowwise(C.byref(make(1)), scales, C.byref(h)) == 2
+    assert L.lib.bert_b200_encoder_create_rowwise(C.byref(cfg), None, C.byref(h)) == 2
+    assert L.lib.bert_b200_encoder_create_rowwise(None, scales, C.byref(h)) == 2
+    scales[1].wt_ffn2 = None
+    assert L.lib.bert_b200_encoder_create_rowwise(C.byref(cfg), scales, C.byref(h)) == 2
+    assert L.lib.bert_b200_encoder_create(C.byref(cfg), C.byref(h)) == 2                      # without them the steps are needed
