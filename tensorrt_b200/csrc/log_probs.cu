@@ -220,6 +220,10 @@ struct Row
     {
         return lastRow && first + n == nVec ? n - 1 : n;
     }
+    __device__ __forceinline__ bool edge(int vec) const
+    {
+        return vec == 0 || vec == nVec - 1;
+    }
     __device__ __forceinline__ T const* at(int first) const
     {
         return p - mis + static_cast<int64_t>(first) * E;
@@ -358,19 +362,22 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
     for (int i = tid; i < n; i += kThreads)
         most.add(buf[i]);
     float const mine = most.get();
-    float gm = mine;
+    // W > 1: the maxima of 64 groups of threads, two per lane
+    float gm = mine, gm2 = negInf();
     if constexpr (W > 1)
     {
+        constexpr int kGroup = kThreads / 64;
 #pragma unroll
-        for (int o = 1; o < W; o *= 2)
+        for (int o = 1; o < kGroup; o *= 2)
             gm = maxNan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-        if (lane % W == 0)
-            groupMax[tid / W] = gm;
+        if (lane % kGroup == 0)
+            groupMax[tid / kGroup] = gm;
         claim();
         sync();
         gm = groupMax[lane];
+        gm2 = groupMax[lane + 32];
     }
-    float const m = warpMaxNan(gm);
+    float const m = warpMaxNan(maxNan(gm, gm2));
     bool const some = m < __int_as_float(0x7f800000) && m != negInf();
     if (tid == 0)
         place.m = m;
@@ -388,15 +395,33 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
         }
         else
         {
-            // the groups' maxima in order: each warp places 32 / W of them
-#pragma unroll
-            for (int j = 0; j < 32 / W; ++j)
+            // The groups' maxima in order, each warp places its share of them: 32 pairs of groups for few tokens (12 values are at least the
+            // 10th of 32 maxima), all 64 for more (32: 44 values, with 32 maxima 110).
+            if (topK <= 12)
             {
-                int const at = warp * (32 / W) + j;
-                float const x = groupMax[at];
-                int const rank = __popc(__ballot_sync(0xffffffffu, gm > x || (gm == x && lane < at)));
-                if (rank == topK - 1 && lane == 0)
-                    *threshold = x;
+                gm = fmaxf(gm, gm2);
+#pragma unroll
+                for (int j = 0; j < 32 / W; ++j)
+                {
+                    int const at = warp * (32 / W) + j;
+                    float const x = __shfl_sync(0xffffffffu, gm, at);
+                    int const rank = __popc(__ballot_sync(0xffffffffu, gm > x || (gm == x && lane < at)));
+                    if (rank == topK - 1 && lane == 0)
+                        *threshold = x;
+                }
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < 64 / W; ++j)
+                {
+                    int const at = warp * (64 / W) + j;
+                    float const x = groupMax[at];
+                    int const rank = __popc(__ballot_sync(0xffffffffu, gm > x || (gm == x && lane < at)))
+                        + __popc(__ballot_sync(0xffffffffu, gm2 > x || (gm2 == x && lane + 32 < at)));
+                    if (rank == topK - 1 && lane == 0)
+                        *threshold = x;
+                }
             }
         }
     }
@@ -408,6 +433,7 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
         // The warp looks through the vectors of its threads that have such values, a thread's at a time, two lanes per vector: candidates are
         // listed; the part's maxima are counted and no longer among the others.
         uint32_t hits = __ballot_sync(0xffffffffu, mine >= thr && mine != negInf());
+        int ties = 0;
         for (; hits != 0; hits &= hits - 1)
             for (int i = warp * 32 + __ffs(hits) - 1 + (lane >> 1) * kThreads; i < n; i += 16 * kThreads)
             {
@@ -415,12 +441,13 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
                 uint2 const half = *reinterpret_cast<uint2 const*>(e);
                 if (Vec<T>::most(make_uint4(half.x, half.y, half.x, half.y)) < thr)
                     continue;
+                bool const list = topK > 0 && *static_cast<int32_t volatile*>(&place.listed) <= Place<W>::kCap; // beyond, only that it is so counts
                 for (int j = 0; j < E / 2; ++j)
                 {
                     float const x = static_cast<float>(e[j]);
                     if (x >= thr && x != negInf())
                     {
-                        if (topK > 0)
+                        if (list)
                         {
                             int const at = atomicAdd(&place.listed, 1);
                             if (at < Place<W>::kCap)
@@ -429,11 +456,13 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
                         if (x == m)
                         {
                             e[j] = static_cast<T>(negInf());
-                            atomicAdd(&place.ties, 1);
+                            ++ties;
                         }
                     }
                 }
             }
+        if (ties > 0)
+            atomicAdd(&place.ties, ties);
         __syncwarp();
     }
     Sums sums;
@@ -480,10 +509,26 @@ struct Result
     uint64_t key = 0; // of this lane's place among the likely tokens, 0: none
     bool bad = false; // a NaN or +infinity has been seen
 
-    // One key per lane (0: none) to the likely tokens.
+    // One key per lane (0: none; none that is there already) to the likely tokens.
     __device__ __forceinline__ void insert(uint64_t k, int topK, int lane)
     {
         uint32_t todo = __ballot_sync(0xffffffffu, k > __shfl_sync(0xffffffffu, key, topK - 1));
+        if (__popc(todo) > 8)
+        {
+            // sorted among each other, then the better of the i-th best here and the i-th worst there: twenty exchanges instead of a chain of
+            // shuffles for each key (32 keys 1.9 us)
+#pragma unroll
+            for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+                for (int o = size / 2; o > 0; o /= 2)
+                    k = exchange(k, o, ((lane & o) == 0) == ((lane & size) == 0 || size == 32));
+            uint64_t const other = __shfl_sync(0xffffffffu, k, 31 - lane);
+            key = other > key ? other : key;
+#pragma unroll
+            for (int o = 16; o > 0; o /= 2)
+                key = exchange(key, o, (lane & o) == 0);
+            return;
+        }
         for (; todo != 0; todo &= todo - 1)
         {
             uint64_t const x = __shfl_sync(0xffffffffu, k, __ffs(todo) - 1);
@@ -491,6 +536,22 @@ struct Result
             uint64_t const before = __shfl_up_sync(0xffffffffu, key, 1);
             key = lane < at ? key : lane == at ? x : before;
         }
+    }
+
+    // The larger or the smaller of this lane's and that of the lane `o` away.
+    static __device__ __forceinline__ uint64_t exchange(uint64_t k, int o, bool larger)
+    {
+        uint64_t const x = __shfl_xor_sync(0xffffffffu, k, o);
+        return (k > x) == larger ? k : x;
+    }
+
+    // The key, or 0 if it is among the likely tokens already. All lanes call it.
+    __device__ __forceinline__ uint64_t unlessThere(uint64_t k, int topK) const
+    {
+        for (int i = 0; i < topK; ++i)
+            if (__shfl_sync(0xffffffffu, key, i) == k)
+                k = 0;
+        return k;
     }
 };
 
@@ -520,16 +581,38 @@ __device__ __forceinline__ void takePlace(Result& res, Place<W>& place, Row<T> c
         }
         res.stat = merge(res.stat, Stat{m, static_cast<float>(place.ties), s, t});
         int const listed = topK > 0 ? place.listed : 0;
-        if (listed <= Place<W>::kCap)
-            for (int i = 0; i < listed; i += 32)
-                res.insert(i + lane < listed ? place.cand[i + lane] : 0ull, topK, lane);
-        else
+        for (int i = 0; i < listed && i < Place<W>::kCap; i += 32)
+            res.insert(i + lane < listed && i + lane < Place<W>::kCap ? place.cand[i + lane] : 0ull, topK, lane);
+        if (listed > Place<W>::kCap)
         {
-            int32_t const begin = max(first * E - row.mis, 0), end = min((first + n) * E - row.mis, vocab);
-            for (int32_t i = begin; i < end; i += 32)
+            // Not all were listed: the part is read again for what is above the last of those found so far, four vectors per lane at a time;
+            // where one of 32 has such values (or may hold values that are not the row's) all of theirs are looked at.
+            T const* const q = row.at(first);
+            for (int i = lane; i - lane < n; i += 4 * 32)
             {
-                float const v = i + lane < end ? static_cast<float>(__ldg(row.p + i + lane)) : negInf();
-                res.insert(v == negInf() ? 0ull : makeKey(v, i + lane), topK, lane);
+                uint4 v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + 32 * j < n && !row.edge(first + i + 32 * j))
+                        v[j] = ldgStream(q + static_cast<int64_t>(i + 32 * j) * E);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    uint64_t const last = __shfl_sync(0xffffffffu, res.key, topK - 1);
+                    int32_t const id = (first + i + 32 * j) * E - row.mis;
+                    bool look = i + 32 * j < n;
+                    if (look && last != 0ull && !row.edge(first + i + 32 * j))
+                    {
+                        float const most = Vec<T>::most(v[j]);
+                        look = most > keyValue(last) || (most == keyValue(last) && id < keyId(last));
+                    }
+                    if (__any_sync(0xffffffffu, look))
+                        for (int e = 0; e < E; ++e)
+                        {
+                            float const x = look && id + e >= 0 && id + e < vocab ? static_cast<float>(__ldg(row.p + id + e)) : negInf();
+                            res.insert(res.unlessThere(x == negInf() ? 0ull : makeKey(x, id + e), topK), topK, lane);
+                        }
+                }
             }
         }
     }
@@ -632,7 +715,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 3) logProbsKernel(LogProbsArgs c
     constexpr int kReaders = W * 32, kAll = kReaders + 32;
     constexpr int E = Vec<T>::kElems;
     __shared__ Place<W> places[2];
-    __shared__ float groupMax[32], threshold;
+    __shared__ float groupMax[64], threshold;
     __shared__ Stat joinStat; // of this CTA, read by the cluster's first
     __shared__ uint64_t joinTop[kMaxTop];
     __shared__ uint32_t joinBad;

@@ -176,23 +176,17 @@ def _here(*tensors):
 
 def _vector(t, n, what):
     """Pointer of a contiguous FP32 vector of n values."""
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous float32 vector of {n} values, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _row_stride(t, what, multiple=1):
     """Row stride of a matrix whose rows are contiguous (views of wider tensors are fine)."""
-    rows, width = t.shape
-    if width > 1 and t.stride(1) != 1:
+    (rows, width), (stride, step) = t.shape, t.stride()
+    if step != 1 and width > 1:
         raise ValueError(f"{what}: the values of a row must be contiguous")
-    return t.stride(0) if rows > 1 else (width + multiple - 1) // multiple * multiple  # of a single row the stride says nothing
-
-
-def _int8_rows(rows, width, device):
-    """INT8 matrix whose rows begin on 16 bytes, as fc_rowwise reads it."""
-    t = torch.empty((rows, (width + 15) & ~15), dtype=torch.int8, device=device)
-    return t if width & 15 == 0 else t[:, :width]
+    return stride if rows > 1 else -(-width // multiple) * multiple  # of a single row the stride says nothing
 
 
 def quantize_rows(x):
@@ -201,19 +195,20 @@ def quantize_rows(x):
     16. Also makes per-channel weights for fc_rowwise out of an [n, k] weight. A row of zeros has scale 0, a row with NaN or infinity
     scale NaN."""
     _here(x)
-    if x.dtype not in (torch.float16, torch.float32):
-        raise ValueError(f"quantize_rows takes float16 or float32, not {x.dtype}")
     if x.dim() != 2:
         if x.dim() == 0 or not x.is_contiguous():
             raise ValueError("quantize_rows: a tensor that is no matrix must be contiguous, with at least one dimension")
         q, scales = quantize_rows(x.view(-1, x.shape[-1]))
         return q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0], scales.view(x.shape[:-1])
+    if x.dtype is not torch.float16 and x.dtype is not torch.float32:
+        raise ValueError(f"quantize_rows takes float16 or float32, not {x.dtype}")
     rows, width = x.shape
-    q = _int8_rows(rows, width, x.device)
-    scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    check(lib.bert_b200_quantize_rows(_stream(), _TYPE_ID[x.dtype], rows, width, x.data_ptr(), _row_stride(x, "quantize_rows"), q.data_ptr(),
-                                      (width + 15) & ~15, scales.data_ptr()), "quantize_rows")
-    return q, scales
+    stride = (width + 15) & ~15
+    q = x.new_empty((rows, stride), dtype=torch.int8)
+    scales = x.new_empty(rows, dtype=torch.float32)
+    check(lib.bert_b200_quantize_rows(_stream(), _TYPE_ID[x.dtype], rows, width, x.data_ptr(), _row_stride(x, "quantize_rows"), q.data_ptr(), stride,
+                                      scales.data_ptr()), "quantize_rows")
+    return (q if stride == width else q[:, :width]), scales
 
 
 def fc_rowwise(a, a_scales, wt, wt_scales, bias=None, activation=ACT_NONE, out_dtype=torch.float16, status=None, out=None):
@@ -221,23 +216,27 @@ def fc_rowwise(a, a_scales, wt, wt_scales, bias=None, activation=ACT_NONE, out_d
     result, any sizes. Rows of A, Wt and `out` begin on 16 bytes (they may be views of wider tensors); without `out`, a result whose rows would
     not is a view of padded rows."""
     _here(a, a_scales, wt, wt_scales, bias, status, out)
-    if a.dtype != torch.int8 or wt.dtype != torch.int8 or a.dim() != 2 or wt.dim() != 2 or a.shape[1] != wt.shape[1]:
+    if a.dtype is not torch.int8 or wt.dtype is not torch.int8 or a.dim() != 2 or wt.dim() != 2 or a.shape[1] != wt.shape[1]:
         raise ValueError(f"fc_rowwise takes int8 matrices [m, k] and [n, k], got {a.dtype} {tuple(a.shape)} and {wt.dtype} {tuple(wt.shape)}")
-    if out_dtype not in (torch.float16, torch.float32):
+    if out_dtype is not torch.float16 and out_dtype is not torch.float32:
         raise ValueError(f"fc_rowwise gives float16 or float32, not {out_dtype}")
     m, k = a.shape
     n = wt.shape[0]
-    per = 16 // out_dtype.itemsize
+    per = 8 if out_dtype is torch.float16 else 4
     if out is None:
         if n % per == 0:
-            out = torch.empty((m, n), dtype=out_dtype, device=a.device)
-        else:  # whole lines of 128 bytes: 640 x 30522 FP32 44 us with rows padded to 16 bytes, 36 us so
-            out = torch.empty((m, -(-n // (8 * per)) * 8 * per), dtype=out_dtype, device=a.device)[:, :n]
-    elif out.dtype != out_dtype or tuple(out.shape) != (m, n):
+            out = a.new_empty((m, n), dtype=out_dtype)
+            ldc = n
+        else:  # whole lines of 128 bytes: 640 x 30522 FP32 44 us with rows padded to 16 bytes, 37 us so
+            ldc = -(-n // (8 * per)) * 8 * per
+            out = a.new_empty((m, ldc), dtype=out_dtype)[:, :n]
+    elif out.dtype is not out_dtype or out.shape != (m, n):
         raise ValueError(f"out must be a {out_dtype} tensor of shape {(m, n)}")
+    else:
+        ldc = _row_stride(out, "out", per)
     p = _lib.FcRowwiseParams(_TYPE_ID[out_dtype], activation, m, n, k, a.data_ptr(), _row_stride(a, "a", 16), _vector(a_scales, m, "a_scales"),
-                             wt.data_ptr(), _row_stride(wt, "wt", 16), _vector(wt_scales, n, "wt_scales"), out.data_ptr(),
-                             _row_stride(out, "out", per), None if bias is None else _vector(bias, n, "bias"), _ptr(status))
+                             wt.data_ptr(), _row_stride(wt, "wt", 16), _vector(wt_scales, n, "wt_scales"), out.data_ptr(), ldc,
+                             None if bias is None else _vector(bias, n, "bias"), _ptr(status))
     check(lib.bert_b200_fc_rowwise(C.byref(p), _stream()), "fc_rowwise")
     return out
 
@@ -247,17 +246,22 @@ def skip_layer_norm_quantize(x, skip, gamma, beta, bias=None, eps=0.0, with_outp
     LayerNorm alone; with_output False: y is None. y has the bits of skip_layer_norm (whose FP16 form has eps 0); the INT8 rows are those
     of the FP32 result before it is rounded to y's type. They feed fc_rowwise where the width is a multiple of 16."""
     _here(x, skip, gamma, beta, bias)
-    ld = x.shape[-1]
-    for t, shape, what in ((skip, x.shape, "skip"), (gamma, (ld,), "gamma"), (beta, (ld,), "beta"), (bias, (ld,), "bias")):
-        if t is not None and (t.dtype != x.dtype or t.shape != shape):
-            raise ValueError(f"skip_layer_norm_quantize: {what} must be {x.dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if x.dtype not in (torch.float16, torch.float32):
-        raise ValueError(f"skip_layer_norm_quantize takes float16 or float32, not {x.dtype}")
+    shape, dtype = x.shape, x.dtype
+    if (dtype is not torch.float16 and dtype is not torch.float32) or not shape:
+        raise ValueError(f"skip_layer_norm_quantize takes float16 or float32 rows, got {dtype} {tuple(shape)}")
+    ld = shape[-1]
+    if skip is not None and (skip.dtype is not dtype or skip.shape != shape):
+        raise ValueError(f"skip_layer_norm_quantize: skip must be {dtype} of shape {tuple(shape)}, got {skip.dtype} {tuple(skip.shape)}")
+    for t in (gamma, beta) if bias is None else (gamma, beta, bias):
+        if t.dtype is not dtype or t.shape != (ld,):
+            raise ValueError(f"skip_layer_norm_quantize: gamma, beta and bias must be {dtype} of shape {(ld,)}, got {t.dtype} {tuple(t.shape)}")
+    x_ptr = _ptr(x)
     y = torch.empty_like(x) if with_output else None
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    check(lib.bert_b200_skip_layer_norm_quantize(_stream(), _TYPE_ID[x.dtype], ld, x.numel(), _ptr(x), _ptr(skip), _ptr(beta), _ptr(gamma), _ptr(y),
-                                                 q.data_ptr(), scales.data_ptr(), _ptr(bias), eps), "skip_layer_norm_quantize")
+    q = torch.empty_like(x, dtype=torch.int8)
+    scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    check(lib.bert_b200_skip_layer_norm_quantize(_stream(), _TYPE_ID[dtype], ld, x.numel(), x_ptr, _ptr(skip), _ptr(beta), _ptr(gamma),
+                                                 None if y is None else y.data_ptr(), q.data_ptr(), scales.data_ptr(), _ptr(bias), eps),
+          "skip_layer_norm_quantize")
     return y, q, scales
 
 
@@ -273,22 +277,22 @@ def token_log_probs(logits, token_ids=None, top_k=0):
     matrix or a view with a row stride. token_ids: int32 [rows, tokens] or [rows]; ids outside the vocabulary have probability 0. Tokens of
     logit -inf are no alternatives (ids -1 where too few are left); rows with NaN or +inf give NaN."""
     _here(logits, token_ids)
-    if logits.dtype not in (torch.float16, torch.float32) or logits.dim() != 2:
+    if (logits.dtype is not torch.float16 and logits.dtype is not torch.float32) or logits.dim() != 2:
         raise ValueError(f"token_log_probs takes float16 or float32 logits [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
     rows, vocab = logits.shape
-    tokens = 0
+    tokens, lp, ids, top = 0, None, None, None
     if token_ids is not None:
-        if token_ids.dtype != torch.int32 or token_ids.dim() not in (1, 2) or token_ids.shape[0] != rows or not token_ids.is_contiguous():
+        if token_ids.dtype is not torch.int32 or token_ids.dim() not in (1, 2) or token_ids.shape[0] != rows or not token_ids.is_contiguous():
             raise ValueError(f"token_ids must be a contiguous int32 tensor [{rows}, tokens] or [{rows}], got {token_ids.dtype} {tuple(token_ids.shape)}")
         tokens = token_ids.shape[1] if token_ids.dim() == 2 else 1
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    lp = torch.empty(token_ids.shape, **f32) if token_ids is not None else None
-    entropy = torch.empty((rows,), **f32)
-    ids = torch.empty((rows, top_k), dtype=torch.int32, device=logits.device) if top_k > 0 else None
-    top = torch.empty((rows, top_k), **f32) if top_k > 0 else None
+        lp = torch.empty_like(token_ids, dtype=torch.float32)
+    entropy = logits.new_empty(rows, dtype=torch.float32)
+    if top_k > 0:
+        ids = logits.new_empty((rows, top_k), dtype=torch.int32)
+        top = torch.empty_like(ids, dtype=torch.float32)
     p = _lib.LogProbsParams(_TYPE_ID[logits.dtype], rows, vocab, logits.data_ptr(), _row_stride(logits, "token_log_probs"), tokens,
                             token_ids.data_ptr() if tokens else None, top_k, lp.data_ptr() if tokens else None, entropy.data_ptr(),
-                            ids.data_ptr() if ids is not None else None, top.data_ptr() if top is not None else None)
+                            None if ids is None else ids.data_ptr(), None if top is None else top.data_ptr())
     check(lib.bert_b200_token_log_probs(C.byref(p), _stream()), "token_log_probs")
     return LogProbs(lp, entropy, ids, top)
 
