@@ -396,8 +396,8 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
         else
         {
             // The groups' maxima in order, each warp places its share of them: 32 pairs of groups for few tokens (12 values are at least the
-            // 10th of 32 maxima), all 64 for more (32: 44 values, with 32 maxima 110).
-            if (topK <= 12)
+            // 10th of 32 maxima, 31 the 20th), all 64 for more (32: 44 values, with 32 maxima 110).
+            if (topK <= 20)
             {
                 gm = fmaxf(gm, gm2);
 #pragma unroll
@@ -430,37 +430,41 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
     {
         if (W > 1 && topK > 0)
             thr = *threshold;
-        // The warp looks through the vectors of its threads that have such values, a thread's at a time, two lanes per vector: candidates are
-        // listed; the part's maxima are counted and no longer among the others.
+        // The warp looks through the vectors of its threads that have such values, two threads at a time, 16 lanes and one vector per lane for
+        // each (a part has at most 16 vectors per thread): candidates are listed; the part's maxima are counted and no longer among the others.
         uint32_t hits = __ballot_sync(0xffffffffu, mine >= thr && mine != negInf());
         int ties = 0;
-        for (; hits != 0; hits &= hits - 1)
-            for (int i = warp * 32 + __ffs(hits) - 1 + (lane >> 1) * kThreads; i < n; i += 16 * kThreads)
+        while (hits != 0)
+        {
+            uint32_t const rest = hits & (hits - 1); // without the first
+            uint32_t const own = (lane & 16) ? rest : hits;
+            hits = rest & (rest - 1);
+            int const i = warp * 32 + __ffs(own) - 1 + (lane & 15) * kThreads;
+            if (own == 0 || i >= n)
+                continue;
+            if (Vec<T>::most(buf[i]) < thr)
+                continue;
+            T* const e = reinterpret_cast<T*>(buf + i);
+            bool const list = topK > 0 && *static_cast<int32_t volatile*>(&place.listed) <= Place<W>::kCap; // beyond, only that it is so counts
+            for (int j = 0; j < E; ++j)
             {
-                T* const e = reinterpret_cast<T*>(buf + i) + (lane & 1) * (E / 2);
-                uint2 const half = *reinterpret_cast<uint2 const*>(e);
-                if (Vec<T>::most(make_uint4(half.x, half.y, half.x, half.y)) < thr)
-                    continue;
-                bool const list = topK > 0 && *static_cast<int32_t volatile*>(&place.listed) <= Place<W>::kCap; // beyond, only that it is so counts
-                for (int j = 0; j < E / 2; ++j)
+                float const x = static_cast<float>(e[j]);
+                if (x >= thr && x != negInf())
                 {
-                    float const x = static_cast<float>(e[j]);
-                    if (x >= thr && x != negInf())
+                    if (list)
                     {
-                        if (list)
-                        {
-                            int const at = atomicAdd(&place.listed, 1);
-                            if (at < Place<W>::kCap)
-                                place.cand[at] = makeKey(x, (first + i) * E - row.mis + (lane & 1) * (E / 2) + j);
-                        }
-                        if (x == m)
-                        {
-                            e[j] = static_cast<T>(negInf());
-                            ++ties;
-                        }
+                        int const slot = atomicAdd(&place.listed, 1);
+                        if (slot < Place<W>::kCap)
+                            place.cand[slot] = makeKey(x, (first + i) * E - row.mis + j);
+                    }
+                    if (x == m)
+                    {
+                        e[j] = static_cast<T>(negInf());
+                        ++ties;
                     }
                 }
             }
+        }
         if (ties > 0)
             atomicAdd(&place.ties, ties);
         __syncwarp();
