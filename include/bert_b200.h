@@ -259,7 +259,7 @@ BERT_B200_API int32_t bert_b200_quantize_rows(void* stream, int32_t type_id, int
 /*
  * C[m,n] = act( (sum_k A[m,k] * Wt[n,k]) * a_scales[m] * wt_scales[n] + bias[n] ): INT8 operands with a scale for each row of A (token) and
  * each output channel, INT32 sums (exact; k <= 131071), C FP16 or FP32 (out_type_id 1 or 0), bias FP32 or NULL, act per `activation`.
- * Any m, n and k; lda, ldw, ldc are row strides in elements, each a multiple of 16 bytes; A, Wt, C, wt_scales and bias 16-byte aligned.
+ * Any m, n and k; lda, ldw, ldc are row strides in elements, each a multiple of 16 bytes; A, Wt and C 16-byte aligned.
  * Only the m x n values of C are written. A row of C has the same bits whatever m. With FP16 results the GELU is the fitted form of
  * bert_b200_fc (below FP16 resolution), with FP32 results erff. `status_word` as in bert_b200_fc.
  * ref: none (plugin/fcPlugin/fcPlugin.cpp:551-610 has no INT8 scales)

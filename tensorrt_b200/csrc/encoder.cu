@@ -10,6 +10,7 @@
 #include "common.cuh"
 
 #include <cmath>
+#include <exception>
 #include <mutex>
 #include <new>
 #include <vector>
@@ -218,7 +219,17 @@ static int32_t createEncoder(bert_b200_encoder_config const* cfg, bert_b200_roww
     if (!e)
         B200_FAIL(BERT_B200_FAILURE, "encoder_create: out of host memory");
     e->cfg = *cfg;
-    e->layers.assign(cfg->layers_host, cfg->layers_host + cfg->num_layers);
+    try
+    {
+        e->layers.assign(cfg->layers_host, cfg->layers_host + cfg->num_layers);
+        if (scales)
+            e->scales.assign(scales, scales + cfg->num_layers);
+    }
+    catch (std::exception const&)
+    {
+        delete e;
+        B200_FAIL(BERT_B200_FAILURE, "encoder_create: out of host memory");
+    }
     e->cfg.layers_host = e->layers.data();
     for (auto const& l : e->layers)
     {
@@ -232,7 +243,6 @@ static int32_t createEncoder(bert_b200_encoder_config const* cfg, bert_b200_roww
     if (scales)
     {
         e->rowwise = true;
-        e->scales.assign(scales, scales + cfg->num_layers);
         for (auto const& s : e->scales)
             if (!(s.wt_qkv && s.wt_out && s.wt_ffn1 && s.wt_ffn2))
             {

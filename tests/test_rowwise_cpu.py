@@ -44,7 +44,7 @@ def test_fc_rowwise_refusals():
     assert f(None, None) == 2
     for change in (dict(out_type_id=2), dict(activation=7), dict(m=-1), dict(n=0), dict(k=0), dict(k=131072, lda=131072, ldw=131072), dict(lda=96), dict(ldw=99), dict(ldc=16),
                    dict(lda=104), dict(ldw=120), dict(ldc=20), dict(out_type_id=0, ldc=22), dict(a=None), dict(a_scales=None), dict(wt=None), dict(wt_scales=None), dict(c=None),
-                   dict(a=FAKE + 8), dict(wt=FAKE + 8), dict(c=FAKE + 8), dict(wt_scales=FAKE + 4), dict(bias=FAKE + 4), dict(a_scales=FAKE + 2), dict(m=2 ** 31),
+                   dict(a=FAKE + 8), dict(wt=FAKE + 8), dict(c=FAKE + 8), dict(wt_scales=FAKE + 2), dict(bias=FAKE + 1), dict(a_scales=FAKE + 2), dict(m=2 ** 31),
                    dict(n=2 ** 31, ldc=2 ** 31 + 8)):
         p = L.FcRowwiseParams(*{**good, **change}.values())
         assert f(C.byref(p), None) == 2, change

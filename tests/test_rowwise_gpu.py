@@ -392,3 +392,55 @@ def test_a_block_of_layers(cuda):
     torch.cuda.synchronize()
     now = block()
     assert all(torch.equal(a, b) for a, b in zip(captured, now)) and not torch.equal(now[0], ref[0])
+
+
+def test_scales_and_bias_of_any_alignment(cuda):
+    """Output channels of a larger layer: weights from any row on, with their scales and biases."""
+    import tensorrt_b200 as T
+
+    a, sa, w, sw, b = _fc_case(np.random.default_rng(9), 150, 500, 64)
+    t = lambda x: torch.from_numpy(x).to(cuda)
+    ta, tsa, tw, tsw, tb = (t(x) for x in (a, sa, w, sw, b))
+    whole = T.fc_rowwise(ta, tsa, tw, tsw, tb)
+    for i in (1, 3, 250):
+        assert torch.equal(T.fc_rowwise(ta[i:], tsa[i:], tw[i:], tsw[i:], tb[i:]), whole[i:, i:])
+
+
+def test_threads_and_streams_at_once(cuda):
+    """Calls of different shapes from several threads, each on a stream of its own, give what they give one after the other."""
+    import threading
+
+    import tensorrt_b200 as T
+
+    shapes = [(37, 1024, 1024), (300, 4100, 512), (1000, 5003, 200), (5, 70, 33)]
+    cases = []
+    for m, n, k in shapes:
+        g = torch.Generator(device=cuda).manual_seed(m)
+        x, w = torch.randn((m, k), device=cuda, generator=g).half(), torch.randn((n, k), device=cuda, generator=g).half()
+        cases.append((x, *T.quantize_rows(w), torch.ones(k, device=cuda).half(), torch.zeros(k, device=cuda).half()))
+
+    def call(case):
+        x, w, s, gamma, beta = case
+        _, _, _ = T.skip_layer_norm_quantize(x, x, gamma, beta)
+        q, qs = T.quantize_rows(x)
+        y = T.fc_rowwise(q, qs, w, s, out_dtype=torch.float32)
+        return [q, qs, y, *T.token_log_probs(y, top_k=7)[1:]]
+
+    want = [call(c) for c in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = call(cases[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    failed.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed, failed
