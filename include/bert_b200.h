@@ -417,6 +417,7 @@ typedef struct bert_b200_log_probs_params
     float* entropy;
     int32_t* top_ids;
     float* top_log_probs;
+    uint32_t* status_word; /* may be NULL; as in bert_b200_fc (the row's results are NaN then) */
 } bert_b200_log_probs_params;
 
 BERT_B200_API int32_t bert_b200_token_log_probs(bert_b200_log_probs_params const* params, void* stream);

@@ -52,7 +52,7 @@ class FcRowwiseParams(C.Structure):
 class LogProbsParams(C.Structure):
     _fields_ = [("type_id", i32), ("rows", i64), ("vocab", i32), ("logits", vp), ("logits_stride", i64),
                 ("num_tokens", i32), ("token_ids", vp), ("top_k", i32), ("log_probs", vp), ("entropy", vp),
-                ("top_ids", vp), ("top_log_probs", vp)]
+                ("top_ids", vp), ("top_log_probs", vp), ("status_word", vp)]
 
 
 class LayerWeights(C.Structure):

@@ -12,9 +12,9 @@
 // The k most likely tokens: the k-th largest of 32 groups' maxima is a lower bound of the k-th largest value, so only what is at least that
 // (a few more than k) is handed over. Where that is more than the list holds (hundreds of equal values) the last warp reads the part again.
 // Rows of up to 128 vectors: one warp each, the same steps one after the other.
-// Rows longer than a part: a cluster of CTAs takes the parts at once and joins them through distributed shared memory where that does not
-// take SMs from other rows; otherwise a CTA takes them by turns.
-#include "common.cuh"
+// Rows may be shared by a cluster of CTAs: their last warps hand what they found to the first CTA's through distributed shared memory, by turns in
+// two places again, so that no reading warp waits for another CTA.
+#include "sm100.cuh"
 
 namespace b200
 {
@@ -36,6 +36,7 @@ struct LogProbsArgs
     float* entropy;
     int32_t* topIds;
     float* topLogProbs;
+    uint32_t* statusWord;
 };
 
 __device__ __forceinline__ float negInf()
@@ -205,8 +206,8 @@ struct Row
         : p(static_cast<T const*>(args.logits) + row * args.stride)
         , mis(static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T)))
         , nVec((args.vocab + mis + E - 1) / E)
-        , firstRow(row * args.stride < E)
-        , lastRow((args.rows - 1 - row) * args.stride < E)
+        , firstRow(row < E) // (a stride of one value is the least there is)
+        , lastRow(args.rows - 1 - row < E)
     {
     }
 
@@ -712,26 +713,48 @@ __global__ void __launch_bounds__(32 * kGroups) logProbsWarpKernel(LogProbsArgs 
     }
 }
 
+// What the last warp of a cluster's other CTA hands to that of the first.
+struct Joined
+{
+    Stat stat;
+    uint64_t key[kMaxTop];
+    uint32_t bad;
+};
+
+constexpr int kReadingWarps = 8;
+constexpr int kCtasPerSm = 3;
+constexpr int kPartVecs = 4096; // 64 KB, so that three CTAs fit an SM
+constexpr int kMaxCluster = 4;
+
 // Rows are dealt over clusters of `clusterSize` CTAs, of which a CTA takes every clusterSize-th part of `partVecs` vectors.
 template <typename T, int W>
-__global__ void __launch_bounds__((W + 1) * 32, 3) logProbsKernel(LogProbsArgs const args, int const clusterSize, int const partVecs)
+__global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogProbsArgs const args, int const clusterSize, int const partVecs)
 {
     constexpr int kReaders = W * 32, kAll = kReaders + 32;
     constexpr int E = Vec<T>::kElems;
     __shared__ Place<W> places[2];
     __shared__ float groupMax[64], threshold;
-    __shared__ Stat joinStat; // of this CTA, read by the cluster's first
-    __shared__ uint64_t joinTop[kMaxTop];
-    __shared__ uint32_t joinBad;
+    __shared__ Joined joined[2][kMaxCluster - 1];
+    __shared__ uint64_t joinFull[2], joinFree[2]; // of the first CTA, of the others
+    __shared__ uint32_t abortWord;
     extern __shared__ __align__(16) uint4 buf[];
     int const tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
     int const rank = static_cast<int>(blockIdx.x % clusterSize);
     int64_t const rowStep = gridDim.x / clusterSize;
     int const partStep = clusterSize * partVecs;
     if (tid < 2)
+    {
         places[tid].ties = places[tid].listed = 0;
+        mbarInit(&joinFull[tid], 32 * (clusterSize - 1) + (clusterSize == 1 ? 1 : 0));
+        mbarInit(&joinFree[tid], 1);
+        abortWord = 0;
+    }
+    fenceBarrierInit();
     gridDependencyLaunch();
-    __syncthreads();
+    if (clusterSize > 1)
+        clusterSync();
+    else
+        __syncthreads();
     gridDependencyWait();
 
     int use = 0; // parts of this CTA so far
@@ -743,14 +766,11 @@ __global__ void __launch_bounds__((W + 1) * 32, 3) logProbsKernel(LogProbsArgs c
             int const left = row.nVec - from;
             return left < partVecs ? left > 0 ? left : 0 : partVecs;
         };
+        Row<T> row(args, r < args.rows ? r : 0);
         if (r < args.rows)
-        {
-            Row<T> const row(args, r);
             row.template copy<kReaders>(buf, first, vectors(row, first), tid, tid, args);
-        }
         for (; r < args.rows; r += rowStep, first = rank * partVecs)
         {
-            Row<T> const row(args, r);
             bool const rowsLeft = r + rowStep < args.rows;
             Row<T> const below(args, rowsLeft ? r + rowStep : r);
             int n = vectors(row, first);
@@ -783,67 +803,104 @@ __global__ void __launch_bounds__((W + 1) * 32, 3) logProbsKernel(LogProbsArgs c
                 first = thenFirst;
                 n = sameRow ? thenN : 0;
             }
-            if (clusterSize > 1)
-            {
-                clusterBarrier();
-                clusterBarrier();
-            }
+            row = below;
         }
         for (int i = use < 2 ? 0 : use - 2; i < use; ++i) // the places' last releases
             barSync<kAll>(kBarFree + (i & 1));
-        return;
     }
-
-    for (int64_t r = blockIdx.x / clusterSize; r < args.rows; r += rowStep)
+    else
     {
-        Row<T> const row(args, r);
-        float const tokenLogit = rank == 0 ? loadToken(args, row, r, lane) : negInf();
-        Result res;
-        for (int first = rank * partVecs; first < row.nVec; first += partStep, ++use)
+        bool ok = true;
+        int turn = 0;
+        for (int64_t r = blockIdx.x / clusterSize; r < args.rows; r += rowStep, ++turn)
         {
-            int const n = row.nVec - first < partVecs ? row.nVec - first : partVecs;
-            barSync<kAll>(kBarFull + (use & 1));
-            takePlace<T, W>(res, places[use & 1], row, args.vocab, first, n, args.topK, lane);
-            __syncwarp();
-            barArrive<kAll>(kBarFree + (use & 1));
-        }
-        if (clusterSize > 1)
-        {
-            if (lane == 0)
+            Row<T> const row(args, r);
+            float const tokenLogit = rank == 0 ? loadToken(args, row, r, lane) : negInf();
+            Result res;
+            for (int first = rank * partVecs; first < row.nVec; first += partStep, ++use)
             {
-                joinStat = res.stat;
-                joinBad = res.bad ? 1u : 0u;
+                int const n = row.nVec - first < partVecs ? row.nVec - first : partVecs;
+                barSync<kAll>(kBarFull + (use & 1));
+                takePlace<T, W>(res, places[use & 1], row, args.vocab, first, n, args.topK, lane);
+                __syncwarp();
+                barArrive<kAll>(kBarFree + (use & 1));
             }
-            joinTop[lane] = res.key;
-            __syncwarp();
-            clusterBarrier();
-            if (rank == 0)
-                for (int c = 1; c < clusterSize; ++c)
+            if (clusterSize > 1)
+            {
+                int const place = turn & 1;
+                uint32_t const phase = static_cast<uint32_t>(turn >> 1) & 1u;
+                if (rank != 0)
                 {
-                    float4 const x = ldSharedCluster4(reinterpret_cast<float const*>(&joinStat), c);
-                    res.stat = merge(res.stat, Stat{x.x, x.y, x.z, x.w});
-                    res.bad |= ldSharedCluster(&joinBad, c) != 0;
-                    uint32_t const* const k = reinterpret_cast<uint32_t const*>(&joinTop[lane]);
-                    if (args.topK > 0)
-                        res.insert(static_cast<uint64_t>(ldSharedCluster(k + 1, c)) << 32 | ldSharedCluster(k, c), args.topK, lane);
+                    ok = ok && (turn < 2 || mbarWaitWarp(&joinFree[place], phase ^ 1u, &abortWord, kWaitStageFree));
+                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                    if (ok)
+                    {
+                        Joined& to = joined[place][rank - 1];
+                        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapaShared(&to.key[lane], 0)), "l"(res.key) : "memory");
+                        if (lane == 0)
+                        {
+                            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mapaShared(&to.stat, 0)), "f"(res.stat.m),
+                                "f"(res.stat.count), "f"(res.stat.s), "f"(res.stat.t)
+                                : "memory");
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapaShared(&to.bad, 0)), "r"(res.bad ? 1u : 0u) : "memory");
+                        }
+                        mbarArriveCluster(mapaShared(&joinFull[place], 0));
+                    }
                 }
-            clusterBarrier(); // the others' shared memory has been read
+                else
+                {
+                    ok = ok && mbarWaitWarp(&joinFull[place], phase, &abortWord, kWaitTmaFull);
+                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                    res.bad |= !ok;
+                    for (int c = 1; c < clusterSize && ok; ++c) // their sums in order
+                    {
+                        Joined const& from = joined[place][c - 1];
+                        res.stat = merge(res.stat, from.stat);
+                        res.bad |= from.bad != 0;
+                        if (args.topK > 0)
+                            res.insert(from.key[lane], args.topK, lane);
+                    }
+                    __syncwarp();
+                    if (lane == 0 && ok)
+                        for (int c = 1; c < clusterSize; ++c)
+                            mbarArriveCluster(mapaShared(&joinFree[place], c));
+                }
+            }
+            if (rank == 0)
+                writeRow(args, res, row, r, tokenLogit, lane);
         }
-        if (rank == 0)
-            writeRow(args, res, row, r, tokenLogit, lane);
+        if (lane == 0 && abortWord != 0 && args.statusWord)
+            atomicMax(args.statusWord, abortWord);
     }
+    if (clusterSize > 1)
+        clusterSync(); // the others may still write here, or signal
 }
-
-constexpr int kReadingWarps = 8;
-constexpr int kCtasPerSm = 3;
-constexpr int kPartVecs = 4096; // 64 KB, so that three CTAs fit an SM
 
 // Which kernel, and how many CTAs share a row.
 //  - A warp per row for up to 64 vectors, and for up to 512 where there are rows for many warps: FP16 20000 x 2000 47 us against 118 us with
 //    a CTA per row, 10000 x 4000 35 / 65 us, but 600 x 4000 11.7 / 8.1 us and 100 x 2000 7.0 / 4.8 us; beyond 512, 5000 x 9000 61 / 40 us.
-//  - Two or four CTAs per row while all of them find a place at once and each has at least half a part: FP32 100 x 120000 36 us with one,
-//    23 with two, 17 with four; 200 x 30522 12.6 / 11.3 / 16.9 us; FP16 1 x 30522 6.0 / 5.9 / 6.7 us, 100 x 9000 5.5 / 6.6 / 8.0 us. Eight are
-//    placed late (100 x 30522 FP32 26 us), and so are clusters beyond what fits (640 x 30522 FP32 60 us with two, 28.5 us with one).
+//  - One, two or four CTAs per row, whichever has the shortest way: a CTA's share of a row, what a part costs beside its vectors and what joining
+//    costs (in vectors, from times of single rows), where all clusters find a place at once (2.75 CTAs per SM: more clusters of four
+//    wait for one another). FP32 1 x 120000 19.8 us with one CTA, 13.2 with two, 10.5 with four, 100 x 120000 33 / 21.8 / 18.0 us, 200 x 120000
+//    34 / 24.4 / 32.5 us, 100 x 30522 12.5 / 11.1 / 11.5 us; FP16 1 x 30522 5.7 / 7.1 / 7.9 us; beyond, FP32 500 x 30522 19.5 / 21.5 / 53 us.
+inline int clusterFor(int64_t rows, int vecs, int64_t sms)
+{
+    constexpr int kPart = 600, kJoin = 2000;
+    int best = 1;
+    int bestCost = 0;
+    for (int c = 1; c <= kMaxCluster && (c == 1 || rows * c <= sms * 11 / 4); c *= 2)
+    {
+        int const share = (vecs + c - 1) / c;
+        int const cost = share + kPart * ((share + kPartVecs - 1) / kPartVecs) + kJoin * (c - 1);
+        if (c == 1 || cost < bestCost)
+        {
+            best = c;
+            bestCost = cost;
+        }
+    }
+    return best;
+}
+
 template <typename T>
 int32_t launchLogProbs(LogProbsArgs const& args, cudaStream_t stream)
 {
@@ -862,9 +919,7 @@ int32_t launchLogProbs(LogProbsArgs const& args, cudaStream_t stream)
     else
     {
         static SmemOptIn optIn;
-        int cluster = 1;
-        while (cluster < 4 && args.rows * cluster * 2 <= sms * kCtasPerSm && vecs > kPartVecs / 2 * cluster)
-            cluster *= 2;
+        int const cluster = clusterFor(args.rows, vecs, sms);
         int const share = (vecs + cluster - 1) / cluster;
         int const partVecs = share < kPartVecs ? share : kPartVecs;
         int64_t const most = sms * kCtasPerSm / cluster * cluster, ctas = args.rows * cluster;
@@ -896,11 +951,11 @@ extern "C" int32_t bert_b200_token_log_probs(bert_b200_log_probs_params const* p
     B200_REQUIRE(p->logits && (p->num_tokens == 0 || (p->token_ids && p->log_probs)) && (p->top_k == 0 || (p->top_ids && p->top_log_probs)),
         "token_log_probs: null pointer");
     uintptr_t const elem = p->type_id == BERT_B200_FP16 ? 2 : 4;
-    uintptr_t const words = reinterpret_cast<uintptr_t>(p->token_ids) | reinterpret_cast<uintptr_t>(p->log_probs) | reinterpret_cast<uintptr_t>(p->entropy)
+    uintptr_t const words = reinterpret_cast<uintptr_t>(p->status_word) | reinterpret_cast<uintptr_t>(p->token_ids) | reinterpret_cast<uintptr_t>(p->log_probs) | reinterpret_cast<uintptr_t>(p->entropy)
         | reinterpret_cast<uintptr_t>(p->top_ids) | reinterpret_cast<uintptr_t>(p->top_log_probs);
     B200_REQUIRE(reinterpret_cast<uintptr_t>(p->logits) % elem == 0 && words % 4 == 0, "token_log_probs: a pointer is not aligned to its type");
     LogProbsArgs const args{p->rows, p->vocab, p->logits, p->logits_stride, p->num_tokens, p->token_ids, p->top_k, p->log_probs, p->entropy, p->top_ids,
-        p->top_log_probs};
+        p->top_log_probs, p->status_word};
     auto s = static_cast<cudaStream_t>(stream);
     return p->type_id == BERT_B200_FP16 ? launchLogProbs<__half>(args, s) : launchLogProbs<float>(args, s);
 }

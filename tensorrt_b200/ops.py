@@ -272,11 +272,11 @@ class LogProbs(NamedTuple):
     top_log_probs: torch.Tensor | None
 
 
-def token_log_probs(logits, token_ids=None, top_k=0):
+def token_log_probs(logits, token_ids=None, top_k=0, status=None):
     """Log probabilities of given tokens, entropy and the top_k (at most 32) most likely tokens of each row of FP16/FP32 logits [rows, vocab], a
     matrix or a view with a row stride. token_ids: int32 [rows, tokens] or [rows]; ids outside the vocabulary have probability 0. Tokens of
     logit -inf are no alternatives (ids -1 where too few are left); rows with NaN or +inf give NaN."""
-    _here(logits, token_ids)
+    _here(logits, token_ids, status)
     if (logits.dtype is not torch.float16 and logits.dtype is not torch.float32) or logits.dim() != 2:
         raise ValueError(f"token_log_probs takes float16 or float32 logits [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
     rows, vocab = logits.shape
@@ -292,7 +292,7 @@ def token_log_probs(logits, token_ids=None, top_k=0):
         top = torch.empty_like(ids, dtype=torch.float32)
     p = _lib.LogProbsParams(_TYPE_ID[logits.dtype], rows, vocab, logits.data_ptr(), _row_stride(logits, "token_log_probs"), tokens,
                             token_ids.data_ptr() if tokens else None, top_k, lp.data_ptr() if tokens else None, entropy.data_ptr(),
-                            None if ids is None else ids.data_ptr(), None if top is None else top.data_ptr())
+                            None if ids is None else ids.data_ptr(), None if top is None else top.data_ptr(), _ptr(status))
     check(lib.bert_b200_token_log_probs(C.byref(p), _stream()), "token_log_probs")
     return LogProbs(lp, entropy, ids, top)
 

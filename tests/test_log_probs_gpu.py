@@ -58,9 +58,9 @@ def test_log_probs(cuda, dtype, vocab):
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "fp32"])
-@pytest.mark.parametrize("rows,vocab", [(700, 50), (650, 3000), (1300, 4001), (400, 30522), (310, 70001)])
+@pytest.mark.parametrize("rows,vocab", [(700, 50), (650, 3000), (1300, 4001), (400, 30522), (640, 30522), (310, 70001), (250, 120000)])
 def test_log_probs_many_rows(cuda, dtype, rows, vocab):
-    """More rows than fit the GPU: one CTA per row, also where a row has several parts."""
+    """More rows than fit the GPU: one CTA per row, also where a row has several parts, and clusters that take several rows by turns."""
     import tensorrt_b200 as T
 
     rng = np.random.default_rng(rows)

@@ -56,7 +56,7 @@ def test_token_log_probs_refusals():
     L = _lib()
     f = L.lib.bert_b200_token_log_probs
     names = [n for n, _ in L.LogProbsParams._fields_]
-    good = dict(zip(names, (1, 4, 100, FAKE, 100, 2, FAKE, 5, FAKE, FAKE, FAKE, FAKE)))
+    good = dict(zip(names, (1, 4, 100, FAKE, 100, 2, FAKE, 5, FAKE, FAKE, FAKE, FAKE, None)))
     assert f(None, None) == 2
     for change in (dict(type_id=2), dict(rows=-1), dict(vocab=0), dict(vocab=2 ** 24 + 1, logits_stride=2 ** 25), dict(logits_stride=99), dict(num_tokens=-1), dict(top_k=-1),
                    dict(top_k=33), dict(logits=None), dict(token_ids=None), dict(log_probs=None), dict(top_ids=None), dict(top_log_probs=None), dict(logits=FAKE + 1),
