@@ -117,6 +117,30 @@ def test_quantize_rows_strides_and_alignment(cuda, dtype, pad, offset):
         _check_rows(*T.quantize_rows(view), buf[:, offset:offset + width])
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("width", [1, 5, 300, 505, 510, 513, 770, 1017, 1018, 1025, 1533, 2041, 3000, 4081, 4090, 4095, 4097, 6001, 8185, 8192, 8193])
+def test_quantize_rows_that_begin_anywhere(cuda, dtype, width):
+    """Row strides that are no multiple of 16 bytes, every kernel for few and for many rows; NaN before, between and behind the rows, and what lies between
+    the results' rows, are left alone."""
+    from tensorrt_b200 import _lib
+
+    t, n = TYPES[dtype]
+    rng = np.random.default_rng(width)
+    for rows, pad, offset in ((1, 0, 3), (2, 1, 1), (9, 1, 5), (9, 6, 0), (9, 0, 2), (330, 3, 7)):
+        stride = width + pad
+        buf = np.full(offset + rows * stride + 3, np.nan, dtype=n)
+        x = _rows(rng, rows, width, n)
+        buf[offset:offset + rows * stride].reshape(rows, stride)[:, :width] = x
+        d = torch.from_numpy(buf).to(cuda)
+        ld = (width + 23) // 8 * 8
+        out = torch.full((rows, ld), 99, dtype=torch.int8, device=cuda)
+        scales = torch.full((rows + 1,), 5.0, device=cuda)
+        assert _lib.lib.bert_b200_quantize_rows(torch.cuda.current_stream().cuda_stream, 1 if dtype == "fp16" else 0, rows, width,
+                                                d.data_ptr() + offset * d.element_size(), stride, out.data_ptr(), ld, scales.data_ptr()) == 0
+        _check_rows(out[:, :width], scales[:rows], x)
+        assert (out[:, width:] == 99).all() and scales[rows] == 5
+
+
 def test_quantize_rows_shapes_and_untouched_padding(cuda):
     import ctypes as C
 
