@@ -241,7 +241,192 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<CPL>) skipLnQuantKernel(i
     }
 }
 
-// Any ld, scalar accesses, one warp per row; the row is revisited from L1 / L2 instead of registers.
+// Rows that cannot be read 16 bytes at a time: WPR warps per row, each with NV neighbouring values per lane, 32 apart, in registers, so that the sums
+// can be those of one warp that goes along the row (skip_ln.cu's scalar kernel, to the bit): each warp goes on where the one before it ended.
+// The next row's 16-byte vectors are on their way to shared memory meanwhile, where single values are read from; the parameters are
+// there for the whole launch. Bound by issue slots (some 35 instructions per value). FP16 24576 x 1001 44.8 us (x 1024 34.5 us; 116 us with the kernel below),
+// FP32 12000 x 1001 33.9 us (81 us), FP16 3000 x 4001 43 us (74 us), 37 x 1001 4.5 us (11.4 us).
+template <typename T>
+struct alignas(2 * sizeof(T)) GammaBeta
+{
+    T gamma, beta;
+};
+
+template <typename T>
+__host__ __device__ constexpr int oddRowBytes(int slots) // of a row in shared memory, and what its lanes may read behind it
+{
+    return (slots * static_cast<int>(sizeof(T)) + 31) / 16 * 16;
+}
+
+template <typename T, int NV, int WPR, bool HAS_BIAS>
+__global__ void __launch_bounds__(kThreads, NV <= 8 ? 4 : NV <= 16 ? 3 : 2) skipLnQuantOddKernel(int32_t const ld, int64_t const rows, T const* in, T const* skip,
+    T const* __restrict__ beta, T const* __restrict__ gamma, T const* __restrict__ bias, T* out, float const eps, int8_t* __restrict__ outI8,
+    float* __restrict__ rowScales)
+{
+    constexpr int kRowsPerCta = kWarpsPerCta / WPR;
+    constexpr int kSlots = NV * WPR * 32;
+    constexpr int kSure = WPR == 1 && NV > 8 ? NV - 8 : 0; // of a lane's values, those that every row handled here has
+    constexpr int kRowBytes = oddRowBytes<T>(kSlots);
+    extern __shared__ __align__(16) uint8_t oddSmem[];
+    __shared__ float chain[kRowsPerCta][32];
+    __shared__ float red[kRowsPerCta][2][WPR];
+    GammaBeta<T>* const params = reinterpret_cast<GammaBeta<T>*>(oddSmem);
+    T* const biases = reinterpret_cast<T*>(params + kSlots);
+    int const lane = threadIdx.x & 31;
+    int const warp = threadIdx.x >> 5;
+    int const rowInCta = warp / WPR;
+    int const wInRow = warp % WPR;
+    uint8_t* const bufA = reinterpret_cast<uint8_t*>(biases + kSlots) + rowInCta * 2 * kRowBytes;
+    uint8_t* const bufB = bufA + kRowBytes;
+    int turn = 0;
+    int const first = wInRow * NV * 32 + lane;
+    float const rld = 1.f / static_cast<float>(ld);
+    auto barrier = [&]() {
+        if (WPR == 1)
+            __syncwarp();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + rowInCta), "n"(WPR * 32) : "memory");
+    };
+    auto misOf = [&](T const* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u); };
+    // The vectors that hold the row; of those that reach beyond the matrix only the row's values.
+    auto copy = [&](uint8_t* buf, T const* base, int64_t r) {
+        T const* const p = base + r * ld;
+        uint8_t const* const q = reinterpret_cast<uint8_t const*>(p) - misOf(p);
+        int const n = (misOf(p) + ld * static_cast<int>(sizeof(T)) + 15) / 16;
+        uint8_t const *const begin = reinterpret_cast<uint8_t const*>(base), *const end = reinterpret_cast<uint8_t const*>(base + rows * ld);
+        for (int i = wInRow * 32 + lane; i < n; i += WPR * 32)
+            if (q + 16 * i >= begin && q + 16 * i + 16 <= end)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(buf + 16 * i))), "l"(q + 16 * i)
+                             : "memory");
+            else
+                for (int j = 0; j < 16; j += static_cast<int>(sizeof(T)))
+                {
+                    T const* const x = reinterpret_cast<T const*>(q + 16 * i + j);
+                    if (x >= p && x < p + ld)
+                        *reinterpret_cast<T*>(buf + 16 * i + j) = *x;
+                }
+    };
+    // add(s): s and this lane's values, in order
+    auto along = [&](auto const& add) {
+        if (WPR == 1)
+            return add(0.f);
+#pragma unroll 1
+        for (int w = 0; w < WPR; ++w)
+        {
+            if (w == wInRow)
+                chain[rowInCta][lane] = add(w == 0 ? 0.f : chain[rowInCta][lane]);
+            barrier();
+        }
+        return chain[rowInCta][lane];
+    };
+    auto most = [](float x, float y) { return maxNan(x, y); };
+
+    gridDependencyLaunch();
+    gridDependencyWait();
+    int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerCta + rowInCta;
+    int64_t const step = static_cast<int64_t>(gridDim.x) * kRowsPerCta;
+    if (row < rows)
+    {
+        copy(bufA, in, row);
+        if (skip)
+            copy(bufB, skip, row);
+    }
+    for (int i = threadIdx.x; i < kSlots; i += kThreads)
+    {
+        bool const ok = i < ld;
+        T const zero = static_cast<T>(0.f);
+        params[i] = GammaBeta<T>{ok ? gamma[i] : zero, ok ? beta[i] : zero};
+        if (HAS_BIAS)
+            biases[i] = ok ? bias[i] : zero;
+    }
+    __syncthreads();
+    for (; row < rows; row += step)
+    {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        barrier();
+        T const* const a = reinterpret_cast<T const*>(bufA + misOf(in + row * ld)) + first;
+        T const* const b = skip ? reinterpret_cast<T const*>(bufB + misOf(skip + row * ld)) + first : nullptr;
+        // f(j, whether the row has this lane's value j); of several warps all but the last have all of theirs
+        auto each = [&](auto const& f) {
+            if (WPR > 1 && (wInRow + 1) * NV * 32 <= ld)
+            {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    f(j, true);
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    f(j, j < kSure || first + 32 * j < ld);
+            }
+        };
+        float x[NV / 8][8];
+        each([&](int j, bool ok) { x[j / 8][j % 8] = ok ? static_cast<float>(a[32 * j]) : 0.f; });
+        if (b)
+            each([&](int j, bool ok) { x[j / 8][j % 8] += ok ? static_cast<float>(b[32 * j]) : 0.f; });
+        if (HAS_BIAS)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                x[j / 8][j % 8] += static_cast<float>(biases[first + 32 * j]);
+        barrier(); // the row's buffers are read, `chain` as well
+        if (row + step < rows)
+        {
+            copy(bufA, in, row + step);
+            if (skip)
+                copy(bufB, skip, row + step);
+        }
+        float const mu = __fmul_rn(warpSum(along([&](float s) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                s += x[j / 8][j % 8];
+            return s;
+        })), rld);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            x[j / 8][j % 8] -= mu;
+        if (WPR > 1)
+            barrier(); // `chain` has been read
+        float const rsigma = rsqrtf(warpSum(along([&](float q) {
+            each([&](int j, bool ok) {
+                if (ok)
+                    q = fmaf(x[j / 8][j % 8], x[j / 8][j % 8], q);
+            });
+            return q;
+        })) * rld + eps);
+        float largest = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+        {
+            GammaBeta<T> const p = params[first + 32 * j]; // zeros behind the row: 0, or NaN where the row's own are
+            x[j / 8][j % 8] = fmaf(static_cast<float>(p.gamma) * x[j / 8][j % 8], rsigma, static_cast<float>(p.beta));
+            largest = maxNan(largest, fabsf(x[j / 8][j % 8]));
+        }
+        if (out)
+        {
+            T* const y = out + row * ld + first;
+            each([&](int j, bool ok) {
+                if (ok)
+                    y[32 * j] = static_cast<T>(x[j / 8][j % 8]);
+            });
+        }
+        largest = overWarps<WPR>(warpMaxNan(largest), red[rowInCta], rowInCta, wInRow, lane, turn, most);
+        RowScale const scale = makeRowScale(largest);
+        if (wInRow == 0 && lane == 0)
+            rowScales[row] = rowScaleValue(largest);
+        uint32_t w[NV / 8][2];
+#pragma unroll
+        for (int c = 0; c < NV / 8; ++c)
+            quantRowChunk<8, true>(x[c], scale, w[c]);
+        int8_t* const q = outI8 + row * ld + first;
+        each([&](int j, bool ok) {
+            if (ok)
+                q[32 * j] = static_cast<int8_t>(w[j / 8][j / 4 & 1] >> (8 * (j & 3)));
+        });
+    }
+}
+
+// Longer rows, scalar accesses, one warp per row; the row is revisited from L1 / L2 instead of registers.
 template <typename T, bool HAS_BIAS>
 __global__ void __launch_bounds__(kThreads) skipLnQuantScalarKernel(int32_t const ld, int64_t const rows, T const* in, T const* skip,
     T const* __restrict__ beta, T const* __restrict__ gamma, T const* __restrict__ bias, T* out, float const eps, int8_t* __restrict__ outI8,
@@ -321,12 +506,43 @@ int32_t launch(cudaStream_t s, Args<T> const& p)
     return checkLaunch("skipLnQuantKernel");
 }
 
+template <typename T, int NV, int WPR>
+int32_t launchOdd(cudaStream_t s, Args<T> const& p)
+{
+    static SmemOptIn optIn[2];
+    constexpr int kSlots = 32 * NV * WPR, kRowsPerCta = kWarpsPerCta / WPR;
+    constexpr int kSmem = kSlots * 3 * static_cast<int>(sizeof(T)) + kRowsPerCta * 2 * oddRowBytes<T>(kSlots);
+    constexpr int kCtas = kSmem > 110 * 1024 ? 1 : kSmem > 73 * 1024 || NV > 16 ? 2 : NV > 8 ? 3 : 4;
+    cudaError_t const e = launchDependentCluster(&optIn[p.bias ? 1 : 0],
+        p.bias ? skipLnQuantOddKernel<T, NV, WPR, true> : skipLnQuantOddKernel<T, NV, WPR, false>,
+        dim3(gridFor((p.rows + kRowsPerCta - 1) / kRowsPerCta, kCtas)), dim3(kThreads), kSmem, s, 1, p.ld, p.rows, p.in, p.skip, p.beta, p.gamma, p.bias,
+        p.out, p.eps, p.outI8, p.rowScales);
+    if (e != cudaSuccess)
+        B200_FAIL(BERT_B200_CUDA_ERROR, "skipLnQuantOddKernel: %s", cudaGetErrorString(e));
+    return checkLaunch("skipLnQuantOddKernel");
+}
+
 template <typename T>
 int32_t dispatch(cudaStream_t s, Args<T> const& p)
 {
     constexpr int E = 16 / sizeof(T);
     bool const vec = p.ld % E == 0 && p.ld / E <= 32 * 4 * 8 && aligned16(p.in) && aligned16(p.skip) && aligned16(p.out) && aligned16(p.beta)
         && aligned16(p.gamma) && aligned16(p.bias) && reinterpret_cast<uintptr_t>(p.outI8) % E == 0;
+    if (!vec && p.ld <= 32 * 32 * 8)
+    {
+        // as few warps as hold the row, 32 values per lane at most
+#define B200_ODD_CASE(NV, W)                                                                                           \
+    if (p.ld <= 32 * NV * W)                                                                                           \
+        return launchOdd<T, NV, W>(s, p);
+        B200_ODD_CASE(8, 1)
+        B200_ODD_CASE(16, 1)
+        B200_ODD_CASE(24, 1)
+        B200_ODD_CASE(32, 1)
+        B200_ODD_CASE(32, 2)
+        B200_ODD_CASE(32, 4)
+        B200_ODD_CASE(32, 8)
+#undef B200_ODD_CASE
+    }
     if (!vec)
     {
         int const grid = gridFor((p.rows + kWarpsPerCta - 1) / kWarpsPerCta, 8);

@@ -349,6 +349,51 @@ def test_skip_layer_norm_quantize(cuda, dtype, ld):
             assert np.abs(y.double().cpu().numpy() - ref).max() <= (H if dtype == "fp16" else 0) * np.abs(ref).max() + 64 * U * (1 + np.abs(ref).max())
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("ld", [3, 31, 255, 257, 510, 513, 767, 769, 770, 1001, 1023, 1025, 2041, 2047, 2049, 4001, 4095, 4097, 8001, 8191, 8193])
+def test_skip_layer_norm_quantize_odd_widths(cuda, dtype, ld):
+    """Rows that begin at any value, tensors that do too, few and many of them, in place: y to the bit that of skip_layer_norm, the INT8 rows those of any
+    other call with the same values; what lies around the tensors is left alone."""
+    import tensorrt_b200 as T
+
+    t, n = TYPES[dtype]
+    gen = torch.Generator(device=cuda).manual_seed(ld)
+    eps = 0.0 if dtype == "fp16" else float(np.finfo(np.float32).eps)
+
+    def tensor(shape, offset, of=None):
+        """`shape` values that begin `offset` values behind a multiple of 16 bytes, between NaN."""
+        size = int(np.prod(shape))
+        buf = torch.full((offset + size + 9,), float("nan"), dtype=t, device=cuda)
+        buf[offset:offset + size] = (torch.randn(size, device=cuda, generator=gen) if of is None else of.flatten()).to(t)
+        return buf[offset:offset + size].view(shape)
+
+    for rows, skipped, biased in ((1, True, False), (7, True, True), (45, False, True), (1500 if ld < 1100 else 700, True, True)):
+        x, s = tensor((rows, ld), rows % 5), tensor((rows, ld), 3) if skipped else None
+        g, b, bi = tensor((ld,), 1), tensor((ld,), 0), tensor((ld,), 2) if biased else None
+        y, q, scales = T.skip_layer_norm_quantize(x, s, g, b, bi, eps=eps)
+        if skipped:
+            assert torch.equal(y, T.skip_layer_norm(x, s, g, b, bi))
+        else:
+            assert torch.equal(y, T.skip_layer_norm_quantize(x, torch.zeros_like(x), g, b, bi, eps=eps)[0])
+        ref = R.layer_norm(*(None if v is None else v.cpu().numpy() for v in (x, s, g, b, bi)), eps)
+        amax = np.abs(ref).max(axis=1, keepdims=True)
+        # as above, the sums here over up to 256 chained additions
+        err = 288 * U * (1 + np.abs(ref).max())
+        np.testing.assert_allclose(scales.cpu().numpy(), amax[:, 0] / 127, rtol=2 * U, atol=err / 127)
+        assert (np.abs(q.cpu().numpy() - 127 * ref / amax) <= 0.5 + 127 * 2 * err / amax).all()
+        # other places in memory, and in place: the same answers
+        x2 = tensor((rows, ld), 6, x)
+        y2, q2, scales2 = T.skip_layer_norm_quantize(x2, None if s is None else tensor((rows, ld), 0, s), g, b, bi, eps=eps)
+        assert torch.equal(y, y2) and torch.equal(q, q2) and torch.equal(scales, scales2)
+        q3, scales3 = torch.full((rows * ld + 2,), 99, dtype=torch.int8, device=cuda), torch.full((rows + 1,), 5.0, device=cuda)
+        x3 = x2._base.clone()
+        assert T._lib.lib.bert_b200_skip_layer_norm_quantize(
+            torch.cuda.current_stream().cuda_stream, 1 if dtype == "fp16" else 0, ld, rows * ld, x3.data_ptr() + 6 * x3.element_size(), None if s is None else s.data_ptr(),
+            b.data_ptr(), g.data_ptr(), x3.data_ptr() + 6 * x3.element_size(), q3.data_ptr() + 1, scales3.data_ptr(), None if bi is None else bi.data_ptr(), eps) == 0
+        assert torch.equal(x3[6:6 + rows * ld].view(rows, ld), y) and torch.isnan(x3[:6]).all() and torch.isnan(x3[6 + rows * ld:]).all()
+        assert torch.equal(q3[1:-1].view(rows, ld), q) and q3[0] == 99 and q3[-1] == 99 and torch.equal(scales3[:-1], scales) and scales3[-1] == 5
+
+
 def test_skip_layer_norm_quantize_special_rows(cuda):
     import tensorrt_b200 as T
 
