@@ -400,7 +400,7 @@ BERT_B200_API int32_t bert_b200_probe_mma_rate(void* stream, int32_t type_id, in
  * all FP32 (ids int32). A logit of -infinity is a token of probability 0: its log probability is -infinity and it is no alternative;
  * where fewer than top_k tokens are left the rest is -1 / -infinity. A row of nothing but -infinity: log probabilities -infinity, entropy
  * 0, no alternatives. A row with a NaN or +infinity: NaN, ids -1. A token id outside [0, vocab) has probability 0 (-infinity).
- * num_tokens and top_k may be 0; vocab is at most 2^24. Log probabilities keep their digits near 0 (a row that is sure of a token).
+ * num_tokens and top_k may be 0; vocab and num_tokens are at most 2^24, rows less than 2^28. Log probabilities keep their digits near 0 (a row that is sure of a token).
  * ref: none (the reference's plugins end at the encoder's output)
  */
 typedef struct bert_b200_log_probs_params

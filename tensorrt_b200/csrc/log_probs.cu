@@ -948,8 +948,8 @@ extern "C" int32_t bert_b200_token_log_probs(bert_b200_log_probs_params const* p
     B200_REQUIRE(p->rows >= 0 && p->rows < (1ll << 31) / 8 && p->vocab > 0 && p->vocab <= 1 << 24, "token_log_probs: bad sizes rows=%lld vocab=%d (at most %d)",
         static_cast<long long>(p->rows), p->vocab, 1 << 24);
     B200_REQUIRE(p->logits_stride >= p->vocab, "token_log_probs: the logits' row stride is smaller than the vocabulary");
-    B200_REQUIRE(p->num_tokens >= 0 && p->top_k >= 0 && p->top_k <= kMaxTop, "token_log_probs: num_tokens=%d, top_k=%d (0 to %d)", p->num_tokens, p->top_k,
-        kMaxTop);
+    B200_REQUIRE(p->num_tokens >= 0 && p->num_tokens <= 1 << 24 && p->top_k >= 0 && p->top_k <= kMaxTop, "token_log_probs: num_tokens=%d (0 to %d), top_k=%d (0 to %d)",
+        p->num_tokens, 1 << 24, p->top_k, kMaxTop);
     B200_REQUIRE(p->num_tokens > 0 || p->top_k > 0 || p->entropy, "token_log_probs: nothing is asked for");
     if (p->rows == 0)
         return BERT_B200_OK;

@@ -67,6 +67,16 @@ def test_token_log_probs_refusals():
     assert f(C.byref(L.LogProbsParams(*{**good, "rows": 0}.values())), None) == 0
 
 
+def test_token_log_probs_sizes_beyond_its_counters_are_refused():
+    L = _lib()
+    good = (1, 4, 100, FAKE, 100, 2, FAKE, 5, FAKE, FAKE, FAKE, FAKE, None)
+    names = [n for n, _ in L.LogProbsParams._fields_]
+    for change in (dict(num_tokens=2 ** 24 + 1), dict(num_tokens=2 ** 31 - 1), dict(rows=2 ** 28)):
+        p = L.LogProbsParams(*{**dict(zip(names, good)), **change}.values())
+        assert L.lib.bert_b200_token_log_probs(C.byref(p), None) == 2, change
+        assert b"token_log_probs" in L.lib.bert_b200_last_error()
+
+
 def test_tensors_off_the_gpu_are_refused():
     import tensorrt_b200 as T
 
