@@ -56,12 +56,23 @@ __device__ __forceinline__ float exp2Approx(float x)
     return y;
 }
 
-// Larger values first, of equal ones (-0 equals 0) the lower id; never 0.
-__device__ __forceinline__ uint64_t makeKey(float x, int32_t id)
+// Whole numbers in the order of the values (-0 equals 0), and back.
+__device__ __forceinline__ uint32_t orderOf(float x)
 {
     int32_t const b = __float_as_int(x + 0.f);
-    uint32_t const order = static_cast<uint32_t>(b ^ ((b >> 31) & 0x7fffffff)) ^ 0x80000000u;
-    return static_cast<uint64_t>(order) << 32 | (0xffffffffu - static_cast<uint32_t>(id));
+    return static_cast<uint32_t>(b ^ ((b >> 31) & 0x7fffffff)) ^ 0x80000000u;
+}
+__device__ __forceinline__ float valueOf(uint32_t order)
+{
+    int32_t const o = static_cast<int32_t>(order ^ 0x80000000u);
+    return __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
+}
+constexpr uint32_t kOrderNegInf = 0x007fffffu;
+
+// Larger values first, of equal ones the lower id; never 0.
+__device__ __forceinline__ uint64_t makeKey(float x, int32_t id)
+{
+    return static_cast<uint64_t>(orderOf(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(id));
 }
 __device__ __forceinline__ int32_t keyId(uint64_t k)
 {
@@ -69,8 +80,7 @@ __device__ __forceinline__ int32_t keyId(uint64_t k)
 }
 __device__ __forceinline__ float keyValue(uint64_t k)
 {
-    int32_t const o = static_cast<int32_t>(static_cast<uint32_t>(k >> 32) ^ 0x80000000u);
-    return __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
+    return valueOf(static_cast<uint32_t>(k >> 32));
 }
 
 template <typename T>
@@ -117,6 +127,14 @@ struct Vec<__half>
             __half2 const m = __hmax2_nan(a, b);
             return maxNan(__low2float(m), __high2float(m));
         }
+        __device__ __forceinline__ float getA() const // of one half of the values
+        {
+            return maxNan(__low2float(a), __high2float(a));
+        }
+        __device__ __forceinline__ float getB() const // of the other
+        {
+            return maxNan(__low2float(b), __high2float(b));
+        }
     };
 };
 template <>
@@ -152,6 +170,14 @@ struct Vec<float>
         __device__ __forceinline__ float get() const
         {
             return maxNan(a, b);
+        }
+        __device__ __forceinline__ float getA() const
+        {
+            return a;
+        }
+        __device__ __forceinline__ float getB() const
+        {
+            return b;
         }
     };
 };
@@ -392,12 +418,26 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
     {
         if constexpr (W == 1)
         {
-            // the largest is taken out topK - 1 times
-            float rest = gm;
-            for (int j = 1; j < topK; ++j)
-                if (__ffs(__ballot_sync(0xffffffffu, rest == warpMaxNan(rest))) - 1 == lane)
-                    rest = negInf();
-            thr = warpMaxNan(rest);
+            if (topK <= 12)
+            {
+                // the largest of the lanes' maxima is taken out topK - 1 times
+                float rest = gm;
+                for (int j = 1; j < topK; ++j)
+                    if (__ffs(__ballot_sync(0xffffffffu, rest == warpMaxNan(rest))) - 1 == lane)
+                        rest = negInf();
+                thr = warpMaxNan(rest);
+            }
+            else
+            {
+                // The maxima of two halves of each lane's values, the topK-th of the 64 to 16 binary places: of 32 maxima the last would leave more
+                // than the list holds (20000 x 2000 FP16, top 32: 442 -> 71 us; 7079 x 231 FP32 48 -> 13.5 us).
+                uint32_t const a = orderOf(most.getA()), b = orderOf(most.getB());
+                uint32_t at = 0;
+                for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+                    if (__popc(__ballot_sync(0xffffffffu, a >= (at | bit))) + __popc(__ballot_sync(0xffffffffu, b >= (at | bit))) >= topK)
+                        at |= bit;
+                thr = valueOf(at > kOrderNegInf ? at : kOrderNegInf);
+            }
         }
         else
         {
@@ -436,20 +476,11 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
     {
         if (W > 1 && topK > 0)
             thr = *threshold;
-        // The warp looks through the vectors of its threads that have such values, two threads at a time, 16 lanes and one vector per lane for
-        // each (a part has at most 16 vectors per thread): candidates are listed; the part's maxima are counted and no longer among the others.
-        uint32_t hits = __ballot_sync(0xffffffffu, mine >= thr && mine != negInf());
+        // Candidates are listed; the part's maxima are counted and no longer among the others.
         int ties = 0;
-        while (hits != 0)
-        {
-            uint32_t const rest = hits & (hits - 1); // without the first
-            uint32_t const own = (lane & 16) ? rest : hits;
-            hits = rest & (rest - 1);
-            int const i = warp * 32 + __ffs(own) - 1 + (lane & 15) * kThreads;
-            if (own == 0 || i >= n)
-                continue;
+        auto look = [&](int i) {
             if (Vec<T>::most(buf[i]) < thr)
-                continue;
+                return;
             T* const e = reinterpret_cast<T*>(buf + i);
             bool const list = topK > 0 && *static_cast<int32_t volatile*>(&place.listed) <= Place<W>::kCap; // beyond, only that it is so counts
             for (int j = 0; j < E; ++j)
@@ -470,7 +501,22 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
                     }
                 }
             }
-        }
+        };
+        uint32_t hits = __ballot_sync(0xffffffffu, mine >= thr && mine != negInf()); // the threads that have such values
+        // Short rows, of which many threads have some: every thread its own vectors.
+        if (W == 1 && 2 * ((n + kThreads - 1) / kThreads) < __popc(hits))
+            for (int i = tid; i < n; i += kThreads)
+                look(i);
+        else // the warp looks through two threads' vectors at a time, 16 lanes and one vector per lane for each (a part has at most 16 per thread)
+            while (hits != 0)
+            {
+                uint32_t const rest = hits & (hits - 1); // without the first
+                uint32_t const own = (lane & 16) ? rest : hits;
+                hits = rest & (rest - 1);
+                int const i = warp * 32 + __ffs(own) - 1 + (lane & 15) * kThreads;
+                if (own != 0 && i < n)
+                    look(i);
+            }
         if (ties > 0)
             atomicAdd(&place.ties, ties);
         __syncwarp();
@@ -525,13 +571,19 @@ struct Result
         uint32_t todo = __ballot_sync(0xffffffffu, k > __shfl_sync(0xffffffffu, key, topK - 1));
         if (__popc(todo) > 8)
         {
-            // sorted among each other, then the better of the i-th best here and the i-th worst there: twenty exchanges instead of a chain of
-            // shuffles for each key (32 keys 1.9 us)
+            // Sorted among each other, then the better of the i-th best here and the i-th worst there: twenty exchanges instead of a chain of
+            // shuffles for each key (32 keys 1.9 us). The first keys need no second half, 16 of them ten exchanges.
 #pragma unroll
-            for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-                for (int o = size / 2; o > 0; o /= 2)
-                    k = exchange(k, o, ((lane & o) == 0) == ((lane & size) == 0 || size == 32));
+            for (int size = 2; size <= 16; size *= 2)
+                sortStep(k, size, lane);
+            bool const first = __shfl_sync(0xffffffffu, key, 0) == 0;
+            if (!first || __any_sync(0xffffffffu, lane >= 16 && k != 0))
+                sortStep(k, 32, lane);
+            if (first)
+            {
+                key = k;
+                return;
+            }
             uint64_t const other = __shfl_sync(0xffffffffu, k, 31 - lane);
             key = other > key ? other : key;
 #pragma unroll
@@ -546,6 +598,14 @@ struct Result
             uint64_t const before = __shfl_up_sync(0xffffffffu, key, 1);
             key = lane < at ? key : lane == at ? x : before;
         }
+    }
+
+    // Runs of `size` keys, each of which rises and falls, become sorted: largest first in every other one, and in the last step.
+    static __device__ __forceinline__ void sortStep(uint64_t& k, int size, int lane)
+    {
+#pragma unroll
+        for (int o = size / 2; o > 0; o /= 2)
+            k = exchange(k, o, ((lane & o) == 0) == ((lane & size) == 0 || size == 32));
     }
 
     // The larger or the smaller of this lane's and that of the lane `o` away.

@@ -69,6 +69,26 @@ def test_log_probs_many_rows(cuda, dtype, rows, vocab):
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("vocab", [17, 33, 64, 130, 231, 281, 504, 1500, 3500])
+def test_log_probs_most_tokens_of_short_rows(cuda, dtype, vocab):
+    """As many likely tokens as there may be of rows that one warp has: random, sorted, of few different values, mostly masked."""
+    import tensorrt_b200 as T
+
+    n = TYPES[dtype][1]
+    rng = np.random.default_rng(vocab)
+    rows = 1300 if vocab > 252 else 40
+    x = _logits(rng, rows, vocab, n)
+    x[1:rows:5] = -np.sort(-x[1:rows:5], axis=1)
+    x[2:rows:5] = np.round(x[2:rows:5])
+    x[3:rows:5] = np.where(rng.random(x[3:rows:5].shape) < 0.95, n(-np.inf), x[3:rows:5])
+    x[4:rows:10] = n(0)
+    x[9:rows:10] *= n(-0.0)
+    ids = rng.integers(0, vocab, size=(rows, 1)).astype(np.int32)
+    for top in (12, 13, 16, 17, 32):
+        _check(T, cuda, x, ids, top)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
 @pytest.mark.parametrize("vocab", [40, 999, 5001, 30522, 70000])
 def test_log_probs_special_rows(cuda, dtype, vocab):
     import tensorrt_b200 as T
