@@ -942,8 +942,10 @@ __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogPr
 }
 
 // Which kernel, and how many CTAs share a row.
-//  - A warp per row for up to 64 vectors, and for up to 512 where there are rows for many warps: FP16 20000 x 2000 47 us against 118 us with
-//    a CTA per row, 10000 x 4000 35 / 65 us, but 600 x 4000 11.7 / 8.1 us and 100 x 2000 7.0 / 4.8 us; beyond 512, 5000 x 9000 61 / 40 us.
+//  - A warp per row for up to 64 vectors, for more where there are rows for many warps: FP16 20000 x 2000 47 us against 118 us with
+//    a CTA per row, 10000 x 4000 35 / 65 us, but 600 x 4000 11.7 / 8.1 us and 100 x 2000 7.0 / 4.8 us; beyond 512, 5000 x 9000 61 / 40 us. Up to 224 a second
+//    round of CTAs is enough: 1000 x 1440, top 10, 9.2 / 10.6 us, x 2000 10.8 / 10.3 us. Up to 160 also for more than 20 tokens, since the vectors
+//    are then too few for 64 groups of threads to bound the 32nd value and most are listed: 1 x 832, top 32, 7.4 / 44 us, x 1440 8.1 / 7.2 us.
 //  - One, two or four CTAs per row, whichever has the shortest way: a CTA's share of a row, what a part costs beside its vectors and what joining
 //    costs (in vectors, from times of single rows), where all clusters find a place at once (2.75 CTAs per SM: more clusters of four
 //    wait for one another). FP32 1 x 120000 19.8 us with one CTA, 13.2 with two, 10.5 with four, 100 x 120000 33 / 21.8 / 18.0 us, 200 x 120000
@@ -973,7 +975,7 @@ int32_t launchLogProbs(LogProbsArgs const& args, cudaStream_t stream)
     int const vecs = (args.vocab + E - 1) / E + 1; // a row may begin inside a vector
     int64_t const sms = smCount();
     cudaError_t e;
-    if (vecs <= 64 || (vecs <= 512 && args.rows > 8 * sms))
+    if (vecs <= 64 || (vecs <= 160 && args.topK > 20) || (vecs <= 224 && args.rows > 3 * sms) || (vecs <= 512 && args.rows > 8 * sms))
     {
         constexpr int kGroups = 4;
         static SmemOptIn optIn;
