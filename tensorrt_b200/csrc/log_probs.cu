@@ -516,6 +516,8 @@ __device__ __forceinline__ void readPart(Place<W>& place, float* groupMax, float
                 int const i = warp * 32 + __ffs(own) - 1 + (lane & 15) * kThreads;
                 if (own != 0 && i < n)
                     look(i);
+                if (W == 1 && own != 0 && i + 16 * kThreads < n)
+                    look(i + 16 * kThreads);
             }
         if (ties > 0)
             atomicAdd(&place.ties, ties);
@@ -942,8 +944,9 @@ __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogPr
 }
 
 // Which kernel, and how many CTAs share a row.
-//  - A warp per row for up to 64 vectors, for more where there are rows for many warps: FP16 20000 x 2000 47 us against 118 us with
-//    a CTA per row, 10000 x 4000 35 / 65 us, but 600 x 4000 11.7 / 8.1 us and 100 x 2000 7.0 / 4.8 us; beyond 512, 5000 x 9000 61 / 40 us. Up to 224 a second
+//  - A warp per row for up to 64 vectors, for more where there are rows for many warps: FP16 20000 x 2000 42 us against 118 us with
+//    a CTA per row, 12000 x 4320 28 / 60 us, 2000 x 6400 11.4 / 14.2 us, but 1200 x 6400 9.9 / 9.6 us, 600 x 4000 11.7 / 8.1 us and 100 x 2000 7.0 /
+//    4.8 us; beyond 832 vectors, 2000 x 8000 16.5 / 15.8 us, top 10 25.5 / 20.8 us. Up to 224 a second
 //    round of CTAs is enough: 1000 x 1440, top 10, 9.2 / 10.6 us, x 2000 10.8 / 10.3 us. Up to 160 also for more than 20 tokens, since the vectors
 //    are then too few for 64 groups of threads to bound the 32nd value and most are listed: 1 x 832, top 32, 7.4 / 44 us, x 1440 8.1 / 7.2 us.
 //  - One, two or four CTAs per row, whichever has the shortest way: a CTA's share of a row, what a part costs beside its vectors and what joining
@@ -975,11 +978,12 @@ int32_t launchLogProbs(LogProbsArgs const& args, cudaStream_t stream)
     int const vecs = (args.vocab + E - 1) / E + 1; // a row may begin inside a vector
     int64_t const sms = smCount();
     cudaError_t e;
-    if (vecs <= 64 || (vecs <= 160 && args.topK > 20) || (vecs <= 224 && args.rows > 3 * sms) || (vecs <= 512 && args.rows > 8 * sms))
+    if (vecs <= 64 || (vecs <= 160 && args.topK > 20) || (vecs <= 224 && args.rows > 3 * sms) || (vecs <= 640 && args.rows > 8 * sms)
+        || (vecs <= 832 && args.rows > 12 * sms))
     {
-        constexpr int kGroups = 4;
+        constexpr int kGroups = sizeof(T) == 4 ? 2 : 4; // warps per CTA: FP32 3000 x 1200 8.5 us with four, 7.1 us with two; FP16 12000 x 4000 27.1 / 27.8 us
         static SmemOptIn optIn;
-        int64_t const most = sms * 16, ctas = (args.rows + kGroups - 1) / kGroups;
+        int64_t const most = sms * (64 / kGroups), ctas = (args.rows + kGroups - 1) / kGroups;
         e = launchDependentCluster(&optIn, logProbsWarpKernel<T, kGroups>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(32 * kGroups),
             static_cast<size_t>(vecs) * 16 * kGroups, stream, 1, args, vecs);
     }

@@ -88,6 +88,23 @@ def test_log_probs_most_tokens_of_short_rows(cuda, dtype, vocab):
         _check(T, cuda, x, ids, top)
 
 
+@pytest.mark.parametrize("dtype,vocab", [("fp16", 5111), ("fp16", 6640), ("fp32", 2500), ("fp32", 3320)])
+def test_log_probs_warp_with_many_vectors(cuda, dtype, vocab):
+    """The longest rows that one warp has, more than sixteen vectors of each lane: few candidates in all of its places, many equal ones."""
+    import tensorrt_b200 as T
+
+    n = TYPES[dtype][1]
+    rng = np.random.default_rng(vocab)
+    x = _logits(rng, 1800, vocab, n)
+    x[np.arange(600), rng.integers(0, vocab, size=600)] = 20
+    x[600:900] = np.round(x[600:900])
+    x[900:1000, ::3] = -np.inf
+    x[1000:1010, 4000 % vocab:] = x.max()
+    ids = rng.integers(0, vocab, size=(1800, 2)).astype(np.int32)
+    for top in (0, 3, 32):
+        _check(T, cuda, x, ids, top)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "fp32"])
 @pytest.mark.parametrize("vocab", [40, 999, 5001, 30522, 70000])
 def test_log_probs_special_rows(cuda, dtype, vocab):
