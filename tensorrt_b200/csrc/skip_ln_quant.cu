@@ -90,6 +90,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<CPL>) skipLnQuantKernel(i
     int const wInRow = warp % WPR;
     int const chunksPerRow = ld / E;
     float const rld = 1.f / static_cast<float>(ld);
+    // Where the INT8 rows go does not choose the kernel (y has to have the bits that skip_layer_norm gives): rows at an odd address go out byte by byte.
+    bool const wholeStores = reinterpret_cast<uintptr_t>(outI8) % E == 0;
     gridDependencyLaunch();
     if (blockIdx.x == 0) // usually in DRAM; a prefetch yields no value, whoever may still be writing it
         for (int i = threadIdx.x * (128 / static_cast<int>(sizeof(T))); i < ld; i += kThreads * (128 / static_cast<int>(sizeof(T))))
@@ -232,10 +234,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<CPL>) skipLnQuantKernel(i
             {
                 uint32_t w[E / 4];
                 quantRowChunk<E, true>(y[i], scale, w);
-                if constexpr (E == 8)
-                    stgStream8(outI8 + row * ld + c * E, make_uint2(w[0], w[1]));
+                int8_t* const to = outI8 + row * ld + c * E;
+                if (!wholeStores)
+                {
+#pragma unroll
+                    for (int j = 0; j < E; ++j)
+                        to[j] = static_cast<int8_t>(w[j / 4] >> (8 * (j & 3)));
+                }
+                else if constexpr (E == 8)
+                    stgStream8(to, make_uint2(w[0], w[1]));
                 else
-                    *reinterpret_cast<uint32_t*>(outI8 + row * ld + c * E) = w[0];
+                    *reinterpret_cast<uint32_t*>(to) = w[0];
             }
         }
     }
@@ -527,7 +536,7 @@ int32_t dispatch(cudaStream_t s, Args<T> const& p)
 {
     constexpr int E = 16 / sizeof(T);
     bool const vec = p.ld % E == 0 && p.ld / E <= 32 * 4 * 8 && aligned16(p.in) && aligned16(p.skip) && aligned16(p.out) && aligned16(p.beta)
-        && aligned16(p.gamma) && aligned16(p.bias) && reinterpret_cast<uintptr_t>(p.outI8) % E == 0;
+        && aligned16(p.gamma) && aligned16(p.bias); // the conditions of dispatchSkipLn (skip_ln.cu)
     if (!vec && p.ld <= 32 * 32 * 8)
     {
         // as few warps as hold the row, 32 values per lane at most

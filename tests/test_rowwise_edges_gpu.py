@@ -1,0 +1,34 @@
+"""Row-wise INT8 and log probabilities where the documentation promises more than the sizes in use show."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp16": (torch.float16, np.float16), "fp32": (torch.float32, np.float32)}
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("ld", [8, 64, 248, 256, 520, 768, 1024, 1528, 2048, 4096, 8192])
+@pytest.mark.parametrize("biased", [False, True])
+def test_skip_layer_norm_quantize_rows_at_any_address(cuda, dtype, ld, biased):
+    """Where the INT8 rows are written changes no bit: y is that of skip_layer_norm, rows and scales those of any other place; the bytes around them stay."""
+    import tensorrt_b200 as T
+
+    t, _ = TYPES[dtype]
+    gen = torch.Generator(device=cuda).manual_seed(ld)
+    rnd = lambda *s: torch.randn(s, device=cuda, generator=gen).to(t)
+    eps = 0.0 if dtype == "fp16" else float(np.finfo(np.float32).eps)
+    for rows in (1, 45, 1500):
+        x, s, g, b, bi = rnd(rows, ld), rnd(rows, ld), rnd(ld), rnd(ld), rnd(ld) if biased else None
+        want = T.skip_layer_norm(x, s, g, b, bi)
+        y0, q0, s0 = T.skip_layer_norm_quantize(x, s, g, b, bi, eps=eps)
+        assert torch.equal(y0, want)
+        for offset in (1, 2, 4, 7):
+            y, q, scales = torch.empty_like(x), torch.full((rows * ld + 16,), 99, dtype=torch.int8, device=cuda), torch.empty(rows, device=cuda)
+            assert T._lib.lib.bert_b200_skip_layer_norm_quantize(
+                torch.cuda.current_stream().cuda_stream, 1 if dtype == "fp16" else 0, ld, rows * ld, x.data_ptr(), s.data_ptr(), b.data_ptr(), g.data_ptr(), y.data_ptr(),
+                q.data_ptr() + offset, scales.data_ptr(), None if bi is None else bi.data_ptr(), eps) == 0
+            assert torch.equal(y, want), offset
+            assert torch.equal(q[offset:offset + rows * ld].view(rows, ld), q0) and torch.equal(scales, s0)
+            assert (q[:offset] == 99).all() and (q[offset + rows * ld:] == 99).all()
