@@ -160,6 +160,8 @@ class MaskedLmHead:
 
     def logits(self, hidden):
         """hidden: FP16 [tokens, hidden] -> [tokens, vocab], FP32 (rowwise) or FP16."""
+        import torch
+
         from . import ops
 
         if self.rowwise:
@@ -167,6 +169,10 @@ class MaskedLmHead:
             t = ops.fc_rowwise(q, s, self.dense, self.dense_scales, self.dense_bias, ops.ACT_GELU_ERF)
             _, q, s = ops.skip_layer_norm_quantize(t, None, self.gamma, self.beta, eps=self.eps, with_output=False)
             return ops.fc_rowwise(q, s, self.decoder, self.decoder_scales, self.bias, out_dtype=self.bias.dtype)
+        # ops.fc goes by the type and the width of what it is given: others than the weights' would be read past the weights' end
+        if hidden.dtype is not torch.float16 or hidden.dim() != 2 or hidden.shape[1] != self.dense.shape[1]:
+            raise ValueError(f"hidden states must be float16 [tokens, {self.dense.shape[1]}], got {hidden.dtype} {tuple(hidden.shape)}")
+        ops._here(hidden, self.dense)
         t = ops.fc(hidden, self.dense, self.dense_bias, ops.ACT_GELU_ERF)
         y, _, _ = ops.skip_layer_norm_quantize(t, None, self.gamma, self.beta, eps=self.eps)
         return ops.fc(y, self.decoder, self.bias)[:, :self.vocab]
