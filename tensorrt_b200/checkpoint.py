@@ -139,7 +139,7 @@ class MaskedLmHead:
         from . import ops
 
         p = "cls.predictions."
-        get = lambda *names: next(torch.from_numpy(_np(state_dict[n])) for n in names if n in state_dict).to(device)
+        get = lambda *names: next(torch.from_numpy(np.ascontiguousarray(_np(state_dict[n]))) for n in names if n in state_dict).to(device)
         dense = get(p + "transform.dense.weight")
         decoder = get(p + "decoder.weight", "bert.embeddings.word_embeddings.weight", "embeddings.word_embeddings.weight")
         self.vocab = decoder.shape[0]

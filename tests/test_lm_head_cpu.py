@@ -24,3 +24,18 @@ def test_hidden_states_of_another_type_or_width_are_refused():
             head(bad, top_k=1)
     with pytest.raises(ValueError, match="CUDA"):
         head.logits(torch.zeros(4, 32).half())
+
+
+def test_weights_in_any_order_of_storage():
+    """A checkpoint's arrays may be views (a transposed kernel of another framework): the kernels get contiguous weights of the same values."""
+    from tensorrt_b200.checkpoint import MaskedLmHead
+
+    sd = _state_dict()
+    turned = {k: np.asfortranarray(v) for k, v in sd.items()}
+    turned["cls.predictions.transform.dense.bias"] = np.repeat(sd["cls.predictions.transform.dense.bias"], 2)[::2]
+    turned["cls.predictions.bias"] = np.repeat(sd["cls.predictions.bias"], 2)[::2]
+    turned["bert.embeddings.word_embeddings.weight"] = torch.from_numpy(np.ascontiguousarray(sd["bert.embeddings.word_embeddings.weight"].T)).t()
+    a, b = (MaskedLmHead(d, device="cpu", rowwise=False) for d in (sd, turned))
+    for name in ("dense", "dense_bias", "gamma", "beta", "decoder", "bias"):
+        x, y = getattr(a, name), getattr(b, name)
+        assert torch.equal(x, y) and y.is_contiguous(), name
