@@ -139,7 +139,11 @@ class MaskedLmHead:
         from . import ops
 
         p = "cls.predictions."
-        get = lambda *names: next(torch.from_numpy(np.ascontiguousarray(_np(state_dict[n]))) for n in names if n in state_dict).to(device)
+
+        def get(*names):  # the first of them that is there
+            name = next((n for n in names if n in state_dict), names[-1])
+            return torch.from_numpy(np.ascontiguousarray(_np(state_dict[name]))).to(device)
+
         dense = get(p + "transform.dense.weight")
         decoder = get(p + "decoder.weight", "bert.embeddings.word_embeddings.weight", "embeddings.word_embeddings.weight")
         self.vocab = decoder.shape[0]

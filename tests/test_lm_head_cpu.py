@@ -39,3 +39,13 @@ def test_weights_in_any_order_of_storage():
     for name in ("dense", "dense_bias", "gamma", "beta", "decoder", "bias"):
         x, y = getattr(a, name), getattr(b, name)
         assert torch.equal(x, y) and y.is_contiguous(), name
+
+
+@pytest.mark.parametrize("name", ["transform.dense.weight", "transform.LayerNorm.bias", "bias"])
+def test_a_missing_weight_is_named(name):
+    from tensorrt_b200.checkpoint import MaskedLmHead
+
+    sd = _state_dict()
+    del sd["cls.predictions." + name]
+    with pytest.raises(KeyError, match="cls.predictions." + name):
+        MaskedLmHead(sd, device="cpu", rowwise=False)
