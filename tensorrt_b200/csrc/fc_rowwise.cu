@@ -18,8 +18,8 @@ int32_t fcRowwiseRun(bert_b200_fc_rowwise_params const& r, cudaStream_t s, bool 
         return BERT_B200_OK;
     B200_REQUIRE(r.a && r.a_scales && r.wt && r.wt_scales && r.c, "fc_rowwise: null pointer");
     int64_t const outElem = r.out_type_id == BERT_B200_FP16 ? 2 : 4;
+    B200_REQUIRE(r.lda < (1ll << 40) && r.ldw < (1ll << 40) && r.ldc < (1ll << 40) / outElem, "fc_rowwise: row strides exceed the 40 bits of a tensor map");
     B200_REQUIRE(r.lda % 16 == 0 && r.ldw % 16 == 0 && r.ldc * outElem % 16 == 0, "fc_rowwise: row strides of A, Wt and C must be multiples of 16 bytes");
-    B200_REQUIRE(r.lda < (1ll << 40) && r.ldw < (1ll << 40) && r.ldc * outElem < (1ll << 40), "fc_rowwise: row strides exceed the 40 bits of a tensor map");
     B200_REQUIRE(aligned16(r.a) && aligned16(r.wt) && aligned16(r.c), "fc_rowwise: A, Wt and C must be 16-byte aligned");
     B200_REQUIRE((reinterpret_cast<uintptr_t>(r.a_scales) | reinterpret_cast<uintptr_t>(r.wt_scales) | reinterpret_cast<uintptr_t>(r.bias)) % 4 == 0,
         "fc_rowwise: a_scales, wt_scales or bias is not aligned to its type");
