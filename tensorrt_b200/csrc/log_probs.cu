@@ -12,8 +12,8 @@
 // The k most likely tokens: the k-th largest of 32 or 64 groups' maxima is a lower bound of the k-th largest value, so only what is at least that
 // (a few more than k) is handed over. Where that is more than the list holds (hundreds of equal values) the last warp reads the part again.
 // Short rows: one warp each, the same steps one after the other.
-// Rows may be shared by a cluster of CTAs: their last warps hand what they found to the first CTA's through distributed shared memory, by turns in
-// two places again, so that no reading warp waits for another CTA.
+// Few rows may be shared by a cluster of CTAs each: their last warps hand what they found to the first CTA's through distributed shared memory. Such
+// a cluster has one row only (clusterFor), so no place there is used twice.
 //
 // Bound by issue slots: of some 10000 warp instructions of a row of 30522 halves, 4000 are exponentials (34 per eight values: conversion, one
 // multiply-add, ex2, two sums, clamp), 700 the maximum, 900 copies, the rest per row and warp; 0.60 of the slots are used with 27 warps per SM. 3686 x
@@ -793,7 +793,8 @@ constexpr int kCtasPerSm = 3;
 constexpr int kPartVecs = 4096; // 64 KB, so that three CTAs fit an SM
 constexpr int kMaxCluster = 4;
 
-// Rows are dealt over clusters of `clusterSize` CTAs, of which a CTA takes every clusterSize-th part of `partVecs` vectors.
+// Rows are dealt over CTAs, each of which has parts of `partVecs` vectors of them; or, with clusterSize > 1, there is a cluster for every row, of which a
+// CTA takes every clusterSize-th part.
 template <typename T, int W>
 __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogProbsArgs const args, int const clusterSize, int const partVecs)
 {
@@ -801,8 +802,8 @@ __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogPr
     constexpr int E = Vec<T>::kElems;
     __shared__ Place<W> places[2];
     __shared__ float groupMax[64], threshold;
-    __shared__ Joined joined[2][kMaxCluster - 1];
-    __shared__ uint64_t joinFull[2], joinFree[2]; // of the first CTA, of the others
+    __shared__ Joined joined[kMaxCluster - 1]; // what the others found, in the first CTA
+    __shared__ uint64_t joinFull;
     __shared__ uint32_t abortWord;
     extern __shared__ __align__(16) uint4 buf[];
     int const tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
@@ -812,10 +813,10 @@ __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogPr
     if (tid < 2)
     {
         places[tid].ties = places[tid].listed = 0;
-        mbarInit(&joinFull[tid], 32 * (clusterSize - 1) + (clusterSize == 1 ? 1 : 0));
-        mbarInit(&joinFree[tid], 1);
         abortWord = 0;
     }
+    if (tid == 0)
+        mbarInit(&joinFull, 32 * (clusterSize - 1) + (clusterSize == 1 ? 1 : 0));
     fenceBarrierInit();
     gridDependencyLaunch();
     if (clusterSize > 1)
@@ -836,19 +837,17 @@ __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogPr
         Row<T> row(args, r < args.rows ? r : 0);
         if (r < args.rows)
             row.template copy<kReaders>(buf, first, vectors(row, first), tid, tid, args);
-        for (; r < args.rows; r += rowStep, first = rank * partVecs)
+        for (; r < args.rows; r += rowStep)
         {
             bool const rowsLeft = r + rowStep < args.rows;
             Row<T> const below(args, rowsLeft ? r + rowStep : r);
             int n = vectors(row, first);
-            if (n == 0 && rowsLeft) // nothing of this row is this CTA's; of the next one it may be
-                below.template copy<kReaders>(buf, first, vectors(below, first), tid, tid, args);
             while (n > 0)
             {
                 // what comes after this part
                 bool const sameRow = first + partStep < row.nVec;
                 Row<T> const then = sameRow ? row : below;
-                int const thenFirst = sameRow ? first + partStep : rank * partVecs;
+                int const thenFirst = sameRow ? first + partStep : 0; // (a CTA that has more than one row has all of their parts)
                 int const thenN = sameRow || rowsLeft ? vectors(then, thenFirst) : 0;
                 int const lo = then.begin(thenFirst), hi = thenN > 0 ? then.end(thenFirst, thenN) : 0;
                 T const* const q = then.at(thenFirst);
@@ -877,9 +876,7 @@ __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogPr
     }
     else
     {
-        bool ok = true;
-        int turn = 0;
-        for (int64_t r = blockIdx.x / clusterSize; r < args.rows; r += rowStep, ++turn)
+        for (int64_t r = blockIdx.x / clusterSize; r < args.rows; r += rowStep)
         {
             Row<T> const row(args, r);
             float const tokenLogit = rank == 0 ? loadToken(args, row, r, lane) : negInf();
@@ -894,43 +891,32 @@ __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogPr
             }
             if (clusterSize > 1)
             {
-                int const place = turn & 1;
-                uint32_t const phase = static_cast<uint32_t>(turn >> 1) & 1u;
                 if (rank != 0)
                 {
-                    ok = ok && (turn < 2 || mbarWaitWarp(&joinFree[place], phase ^ 1u, &abortWord, kWaitStageFree));
-                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
-                    if (ok)
+                    Joined& to = joined[rank - 1];
+                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapaShared(&to.key[lane], 0)), "l"(res.key) : "memory");
+                    if (lane == 0)
                     {
-                        Joined& to = joined[place][rank - 1];
-                        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapaShared(&to.key[lane], 0)), "l"(res.key) : "memory");
-                        if (lane == 0)
-                        {
-                            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mapaShared(&to.stat, 0)), "f"(res.stat.m),
-                                "f"(res.stat.count), "f"(res.stat.s), "f"(res.stat.t)
-                                : "memory");
-                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapaShared(&to.bad, 0)), "r"(res.bad ? 1u : 0u) : "memory");
-                        }
-                        mbarArriveCluster(mapaShared(&joinFull[place], 0));
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mapaShared(&to.stat, 0)), "f"(res.stat.m),
+                            "f"(res.stat.count), "f"(res.stat.s), "f"(res.stat.t)
+                            : "memory");
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapaShared(&to.bad, 0)), "r"(res.bad ? 1u : 0u) : "memory");
                     }
+                    mbarArriveCluster(mapaShared(&joinFull, 0));
                 }
                 else
                 {
-                    ok = ok && mbarWaitWarp(&joinFull[place], phase, &abortWord, kWaitTmaFull);
+                    bool const ok = mbarWaitWarp(&joinFull, 0, &abortWord, kWaitTmaFull);
                     asm volatile("fence.acq_rel.cluster;" ::: "memory");
                     res.bad |= !ok;
                     for (int c = 1; c < clusterSize && ok; ++c) // their sums in order
                     {
-                        Joined const& from = joined[place][c - 1];
+                        Joined const& from = joined[c - 1];
                         res.stat = merge(res.stat, from.stat);
                         res.bad |= from.bad != 0;
                         if (args.topK > 0)
                             res.insert(from.key[lane], args.topK, lane);
                     }
-                    __syncwarp();
-                    if (lane == 0 && ok)
-                        for (int c = 1; c < clusterSize; ++c)
-                            mbarArriveCluster(mapaShared(&joinFree[place], c));
                 }
             }
             if (rank == 0)
@@ -951,8 +937,9 @@ __global__ void __launch_bounds__((W + 1) * 32, kCtasPerSm) logProbsKernel(LogPr
 //    are then too few for 64 groups of threads to bound the 32nd value and most are listed: 1 x 832, top 32, 7.4 / 44 us, x 1440 8.1 / 7.2 us.
 //  - One, two or four CTAs per row, whichever has the shortest way: a CTA's share of a row, what a part costs beside its vectors and what joining
 //    costs (in vectors, from times of single rows), where all clusters find a place at once (2.75 CTAs per SM: more clusters of four
-//    wait for one another). FP32 1 x 120000 19.8 us with one CTA, 13.2 with two, 10.5 with four, 100 x 120000 33 / 21.8 / 18.0 us, 200 x 120000
-//    34 / 24.4 / 32.5 us, 100 x 30522 12.5 / 11.1 / 11.5 us; FP16 1 x 30522 5.7 / 7.1 / 7.9 us; beyond, FP32 500 x 30522 19.5 / 21.5 / 53 us.
+//    wait for one another), so that none has a second row. With one / two / four CTAs, top 5: FP32 1 x 120000 20.4 / 13.5 / 10.0 us, 100 x 120000
+//    34.5 / 22.7 / 17.0 us, 200 x 120000 36 / 24.4 / 33.3 us, 100 x 30522 12.6 / 10.6 / 10.3 us, 140 x 30522 12.7 / 11.4 / 18.9 us; FP16 1 x 30522 5.7 / 6.4 /
+//    6.9 us; beyond, FP32 500 x 30522 19.5 / 28.4 / 47.8 us.
 inline int clusterFor(int64_t rows, int vecs, int64_t sms)
 {
     constexpr int kPart = 600, kJoin = 2000;
@@ -995,8 +982,8 @@ int32_t launchLogProbs(LogProbsArgs const& args, cudaStream_t stream)
         // threads at work to bound the 32nd value (66 -> 28.7 us).
         int const share = (vecs + cluster - 1) / cluster;
         int const parts = (share + kPartVecs - 1) / kPartVecs, partVecs = (share + parts - 1) / parts;
-        int64_t const most = sms * kCtasPerSm / cluster * cluster, ctas = args.rows * cluster;
-        e = launchDependentCluster(&optIn, logProbsKernel<T, kReadingWarps>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)),
+        int64_t const most = sms * kCtasPerSm, ctas = args.rows * cluster;
+        e = launchDependentCluster(&optIn, logProbsKernel<T, kReadingWarps>, dim3(static_cast<unsigned>(cluster > 1 || ctas < most ? ctas : most)),
             dim3((kReadingWarps + 1) * 32), static_cast<size_t>(partVecs) * 16, stream, cluster, args, cluster, partVecs);
     }
     if (e != cudaSuccess)

@@ -32,3 +32,42 @@ def test_skip_layer_norm_quantize_rows_at_any_address(cuda, dtype, ld, biased):
             assert torch.equal(y, want), offset
             assert torch.equal(q[offset:offset + rows * ld].view(rows, ld), q0) and torch.equal(scales, s0)
             assert (q[:offset] == 99).all() and (q[offset + rows * ld:] == 99).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 99, 101, 102, 201, 203, 204])
+@pytest.mark.parametrize("top", [0, 5, 32])
+def test_log_probs_of_rows_that_share_their_ctas_with_none(cuda, dtype, rows, top):
+    """Four or two CTAs for each row, up to as many rows as find places for them, and one beyond: what makes a row special lies in the share of any of them."""
+    import tensorrt_b200 as T
+    from oracle import rowwise_oracle as R
+    from tests.test_log_probs_gpu import _check
+
+    n = TYPES[dtype][1]
+    vocab = 60001 if dtype == "fp32" else 120001
+    rng = np.random.default_rng(rows)
+    base = (2.5 * rng.standard_normal((13, vocab))).astype(n)
+    quarter = vocab // 4
+    for i in range(4):
+        base[i, i * quarter:(i + 1) * quarter] = -np.inf              # nothing left in one share
+        base[4 + i] = -np.inf
+        base[4 + i, i * quarter + 5:i * quarter + 9] = n(1.5)         # all that is left in one share
+    base[8, 3 * quarter + 7] = np.nan
+    base[9, quarter + 7] = np.inf
+    base[10, ::quarter] = 30                                          # the likely ones in different shares
+    base[11] = 0
+    x = base[np.arange(rows) % 13]
+    ids = rng.integers(0, vocab, size=(rows, 2)).astype(np.int32)
+    if rows <= 102:
+        _check(T, cuda, x, ids, top)
+        return
+    # many rows: each as alone
+    t, i = torch.from_numpy(x).to(cuda), torch.from_numpy(ids).to(cuda)
+    got = T.token_log_probs(t, i, top_k=top)
+    ref = R.token_log_probs(x[:13], ids[:13], max(top, 1))
+    for r in range(rows):
+        k = r % 13
+        if top:
+            assert (got.top_ids[r].cpu().numpy() == ref[2][k]).all(), r
+        e = float(got.entropy[r])
+        assert (np.isnan(e) and np.isnan(ref[1][k])) or abs(e - ref[1][k]) <= 5.3e-6 * (1 + 2 * ref[4][k]) + 2.0 ** -22, r
