@@ -280,11 +280,44 @@ __device__ __forceinline__ float warpMaxNan(float v)
     return m;
 }
 
-// 128-bit global load through the read-only path, no L1 allocation (streamed once).
+// Loads of global memory. Ordinary ones, here and in every kernel that calls gridDependencyWait(): a non-coherent load (ld.global.nc, __ldg, a plain read
+// through a `const __restrict__` parameter) promises that nobody writes the data while the kernel runs, so the compiler may move it in front of the wait,
+// where the kernel ahead is still writing. It does so or not as it schedules the rest of a kernel.
+template <typename T>
+__device__ __forceinline__ T ldGlobal(T const* p)
+{
+    static_assert(sizeof(T) == 2 || sizeof(T) == 4 || sizeof(T) == 8 || sizeof(T) == 16, "one load");
+    if constexpr (sizeof(T) == 2)
+    {
+        uint16_t v;
+        asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+        return *reinterpret_cast<T const*>(&v);
+    }
+    else if constexpr (sizeof(T) == 4)
+    {
+        uint32_t v;
+        asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+        return *reinterpret_cast<T const*>(&v);
+    }
+    else if constexpr (sizeof(T) == 8)
+    {
+        uint2 v;
+        asm volatile("ld.global.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+        return *reinterpret_cast<T const*>(&v);
+    }
+    else
+    {
+        uint4 v;
+        asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+        return *reinterpret_cast<T const*>(&v);
+    }
+}
+
+// 128-bit global load, no L1 allocation (streamed once).
 __device__ __forceinline__ uint4 ldgStream(void const* p)
 {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(p));
     return v;
@@ -293,7 +326,7 @@ __device__ __forceinline__ uint4 ldgStream(void const* p)
 // 128-bit global load kept in L1/L2 (parameters, re-used rows).
 __device__ __forceinline__ uint4 ldgKeep(void const* p)
 {
-    return __ldg(reinterpret_cast<uint4 const*>(p));
+    return ldGlobal(static_cast<uint4 const*>(p));
 }
 
 __device__ __forceinline__ void stgStream(void* p, uint4 v)
@@ -307,7 +340,7 @@ __device__ __forceinline__ void stgStream(void* p, uint4 v)
 __device__ __forceinline__ uint2 ldgStream8(void const* p)
 {
     uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
     return v;
 }
 

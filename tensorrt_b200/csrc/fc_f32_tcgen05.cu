@@ -168,7 +168,7 @@ __device__ __forceinline__ bool hasNan(float const* row, int64_t k)
 #pragma unroll 4
     for (int64_t i = (threadIdx.x & 31) * 4; i < k; i += 128)
     {
-        float4 const v = __ldg(reinterpret_cast<float4 const*>(row + i));
+        float4 const v = ldGlobal(reinterpret_cast<float4 const*>(row + i));
         nan |= isnan(v.x) | isnan(v.y) | isnan(v.z) | isnan(v.w);
     }
     return __any_sync(0xffffffffu, nan);
@@ -219,8 +219,8 @@ __device__ __noinline__ void computeAgain(FcF32TcArgs const& p, uint32_t const* 
 #pragma unroll
             for (int j = 0; j < 4; ++j)
             {
-                av[j] = __ldg(reinterpret_cast<float4 const*>(a[j] + k));
-                wv[j] = __ldg(reinterpret_cast<float4 const*>(w[j] + k));
+                av[j] = ldGlobal(reinterpret_cast<float4 const*>(a[j] + k));
+                wv[j] = ldGlobal(reinterpret_cast<float4 const*>(w[j] + k));
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -254,7 +254,7 @@ __device__ __noinline__ void computeAgain(FcF32TcArgs const& p, uint32_t const* 
         if ((lane & 1) == 0 && (mask >> j & 1u) != 0)
         {
             int64_t const n = n0 + c + (j & 3);
-            p.C[(m0 + r + (j >> 2)) * p.ldc + n] = finishF32(p, v[0], p.bias ? __ldg(p.bias + n) : 0.f);
+            p.C[(m0 + r + (j >> 2)) * p.ldc + n] = finishF32(p, v[0], p.bias ? ldGlobal(p.bias + n) : 0.f);
         }
     }
 }
@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(kThreadsF32, 1)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (j < inside)
-                    bias[j] = __ldg(p.bias + n + j);
+                    bias[j] = ldGlobal(p.bias + n + j);
         }
         int r = rank * kRows + static_cast<int>(threadIdx.x) / kPieces;
         float* dst = p.C + (m0 + r) * p.ldc + n;

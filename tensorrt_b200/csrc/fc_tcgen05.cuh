@@ -570,16 +570,16 @@ __global__ void __launch_bounds__(FcTileSmem<BLOCK_M, BLOCK_N, kRowwise>::kThrea
         int const part = (warp - 2) >> 2;
         int const et = static_cast<int>(threadIdx.x) - 64;
         if (args.bias && et < BLOCK_N) // read back by the other epilogue warps
-            sBias[et] = n0 + et < args.N ? __ldg(args.bias + n0 + et) : 0.f;
+            sBias[et] = n0 + et < args.N ? ldGlobal(args.bias + n0 + et) : 0.f;
         float* const sScale = sBias + BLOCK_N;
         float rowScale = 0.f;
         if constexpr (kRowwise)
         {
             if (et < BLOCK_N)
-                sScale[et] = n0 + et < args.N ? __ldg(args.colScale + n0 + et) : 0.f;
+                sScale[et] = n0 + et < args.N ? ldGlobal(args.colScale + n0 + et) : 0.f;
             int64_t const row = static_cast<int64_t>(m0) + quad * kQuadRows + lane;
             if (lane < kQuadRows && row < args.M)
-                rowScale = __ldg(args.rowScale + row);
+                rowScale = ldGlobal(args.rowScale + row);
         }
         asm volatile("bar.sync 1, %0;" ::"n"(L::kEpiWarps * 32) : "memory");
         bool const ok = mbarWaitWarp(accFull, 0, abortFlag, kWaitAccFull);
@@ -940,14 +940,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFcThreads, 1)
             if constexpr (kRowwise)
             {
                 if (rowBase + lane < args.M)
-                    rowScale = __ldg(args.rowScale + rowBase + lane);
+                    rowScale = ldGlobal(args.rowScale + rowBase + lane);
                 float scale[kChunksPerWarp], bias[kChunksPerWarp];
 #pragma unroll
                 for (int i = 0; i < kChunksPerWarp; ++i)
                 {
                     int64_t const c = n0 + (part + i * (kEpilogueWarps / 4)) * 32 + lane;
-                    scale[i] = c < args.N ? __ldg(args.colScale + c) : 0.f;
-                    bias[i] = c < args.N && args.bias ? __ldg(args.bias + c) : 0.f;
+                    scale[i] = c < args.N ? ldGlobal(args.colScale + c) : 0.f;
+                    bias[i] = c < args.N && args.bias ? ldGlobal(args.bias + c) : 0.f;
                 }
                 __syncwarp(); // the tile before has been read
 #pragma unroll

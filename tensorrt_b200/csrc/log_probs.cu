@@ -289,7 +289,7 @@ struct Row
         else
             for (int j = 0; j < E; ++j)
                 if (e0 + j >= 0 && j < left)
-                    reinterpret_cast<T*>(dst)[j] = __ldg(p + e0 + j);
+                    reinterpret_cast<T*>(dst)[j] = ldGlobal(p + e0 + j);
     }
 
     // What of the copied vector is not the row's becomes -infinity.
@@ -681,7 +681,7 @@ __device__ __forceinline__ void takePlace(Result& res, Place<W>& place, Row<T> c
                     if (__any_sync(0xffffffffu, look))
                         for (int e = 0; e < E; ++e)
                         {
-                            float const x = look && id + e >= 0 && id + e < vocab ? static_cast<float>(__ldg(row.p + id + e)) : negInf();
+                            float const x = look && id + e >= 0 && id + e < vocab ? static_cast<float>(ldGlobal(row.p + id + e)) : negInf();
                             res.insert(res.unlessThere(x == negInf() ? 0ull : makeKey(x, id + e), topK), topK, lane);
                         }
                 }
@@ -707,12 +707,26 @@ __device__ __forceinline__ void writeRow(LogProbsArgs const& args, Result const&
     };
     if (lane < args.numTokens)
         args.logProbs[r * args.numTokens + lane] = logProb(tokenLogit);
-#pragma unroll 4
-    for (int j = lane + 32; j < args.numTokens; j += 32)
+    // Many tokens: eight of a lane at a time, the next eight on their way with these ones' logits.
+    constexpr int kAtOnce = 8;
+    auto loadTokens = [&](int j0, int32_t (&token)[kAtOnce]) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            token[i] = j0 + 32 * i < args.numTokens ? ldGlobal(args.tokenIds + r * args.numTokens + j0 + 32 * i) : -1;
+    };
+    int32_t token[kAtOnce];
+    loadTokens(lane + 32, token);
+    for (int j0 = lane + 32; j0 < args.numTokens; j0 += kAtOnce * 32)
     {
-        int32_t const token = __ldg(args.tokenIds + r * args.numTokens + j);
-        float const x = token >= 0 && token < args.vocab ? static_cast<float>(__ldg(row.p + token)) : negInf();
-        args.logProbs[r * args.numTokens + j] = logProb(x);
+        float x[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            x[i] = token[i] >= 0 && token[i] < args.vocab ? static_cast<float>(ldGlobal(row.p + token[i])) : negInf();
+        loadTokens(j0 + kAtOnce * 32, token);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (j0 + 32 * i < args.numTokens)
+                args.logProbs[r * args.numTokens + j0 + 32 * i] = logProb(x[i]);
     }
     if (lane == 0 && args.entropy)
         args.entropy[r] = bad ? nan : none ? 0.f : lse - st.t / (st.count + st.s);
@@ -730,9 +744,9 @@ __device__ __forceinline__ float loadToken(LogProbsArgs const& args, Row<T> cons
 {
     if (lane < args.numTokens)
     {
-        int32_t const token = __ldg(args.tokenIds + r * args.numTokens + lane);
+        int32_t const token = ldGlobal(args.tokenIds + r * args.numTokens + lane);
         if (token >= 0 && token < args.vocab)
-            return static_cast<float>(__ldg(row.p + token));
+            return static_cast<float>(ldGlobal(row.p + token));
     }
     return negInf();
 }

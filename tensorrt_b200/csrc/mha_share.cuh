@@ -52,8 +52,8 @@ struct ShareSmem
 __device__ __forceinline__ int2 fetchGeometry(ShareArgs const& a, int32_t b)
 {
     if (a.fixedLayout())
-        return make_int2(0, a.maskIdx ? __ldg(a.maskIdx + b) : a.S);
-    return make_int2(__ldg(a.cu + b), __ldg(a.cu + b + 1));
+        return make_int2(0, a.maskIdx ? ldGlobal(a.maskIdx + b) : a.S);
+    return make_int2(ldGlobal(a.cu + b), ldGlobal(a.cu + b + 1));
 }
 
 __device__ __forceinline__ Sequence makeSequence(ShareArgs const& a, int2 w)

@@ -174,17 +174,17 @@ __device__ __forceinline__ void tmemStore32(uint32_t taddr, uint32_t const (&r)[
 // First row and valid keys of sequence b.
 template <bool FIXED>
 __device__ __forceinline__ void sequenceOf(
-    int32_t const S, int32_t const* __restrict__ cu, int32_t const* __restrict__ maskIdx, int const b, int32_t& rowBase, int32_t& len)
+    int32_t const S, int32_t const* cu, int32_t const* maskIdx, int const b, int32_t& rowBase, int32_t& len)
 {
     if (FIXED)
     {
         rowBase = 0;
-        len = maskIdx ? min(max(__ldg(maskIdx + b), 0), S) : S;
+        len = maskIdx ? min(max(ldGlobal(maskIdx + b), 0), S) : S;
     }
     else
     {
-        rowBase = __ldg(cu + b);
-        len = min(max(__ldg(cu + b + 1) - rowBase, 0), S);
+        rowBase = ldGlobal(cu + b);
+        len = min(max(ldGlobal(cu + b + 1) - rowBase, 0), S);
     }
 }
 
@@ -995,12 +995,12 @@ __global__ void __launch_bounds__(kShortThreads, 4) mhaShortInt8Kernel(const __g
     if (args.fixedLayout)
     {
         rowBase = 0;
-        len = args.maskIdx ? min(max(__ldg(args.maskIdx + b), 0), args.S) : args.S;
+        len = args.maskIdx ? min(max(ldGlobal(args.maskIdx + b), 0), args.S) : args.S;
     }
     else
     {
-        rowBase = __ldg(args.cu + b);
-        len = min(max(__ldg(args.cu + b + 1) - rowBase, 0), args.S);
+        rowBase = ldGlobal(args.cu + b);
+        len = min(max(ldGlobal(args.cu + b + 1) - rowBase, 0), args.S);
     }
     int32_t const rows = args.fixedLayout ? args.S : len;
     int const q = static_cast<int>(threadIdx.x); // query row = TMEM lane

@@ -52,7 +52,7 @@ struct Chunk<__half>
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (at + j >= 0 && at + j < width)
-                w[j / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<unsigned short const*>(row) + at + j)) << (16 * (j & 1));
+                w[j / 2] |= static_cast<uint32_t>(ldGlobal(reinterpret_cast<unsigned short const*>(row) + at + j)) << (16 * (j & 1));
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
     static __device__ __forceinline__ void trim(uint4& v, int at, int width)
@@ -79,7 +79,7 @@ struct Chunk<float>
     }
     static __device__ __forceinline__ uint4 loadPart(float const* row, int at, int width)
     {
-        auto value = [&](int j) { return at + j >= 0 && at + j < width ? __float_as_uint(__ldg(row + at + j)) : 0u; };
+        auto value = [&](int j) { return at + j >= 0 && at + j < width ? __float_as_uint(ldGlobal(row + at + j)) : 0u; };
         return make_uint4(value(0), value(1), value(2), value(3));
     }
     static __device__ __forceinline__ void trim(uint4& v, int at, int width)
@@ -95,7 +95,7 @@ struct Chunk<float>
 // while this one is quantised: FP32 12000 x 4096 43.0 -> 39.0 us, FP16 12000 x 8192 53.6 -> 51.2 us; FP16 rows of fewer warps lose by the
 // registers it takes (24576 x 1024 14.3 -> 16.7 us).
 template <typename T, int CPL, int WPR>
-__global__ void __launch_bounds__(kThreads) quantizeRowsKernel(int64_t const rows, int32_t const width, T const* __restrict__ in,
+__global__ void __launch_bounds__(kThreads) quantizeRowsKernel(int64_t const rows, int32_t const width, T const* in,
     int64_t const inStride, int8_t* __restrict__ out, int64_t const outStride, float* __restrict__ scales)
 {
     constexpr int E = Chunk<T>::kElems;
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) quantizeRowsKernel(int64_t const row
 // instructions per vector and warp). FP16 24576 x 1001 19.3 us (17.5 us on 16 bytes), x 4095 79 us (52), FP32 12000 x 4097 49 us (39); with one value per
 // lane and load 61, 115 and 59 us, with two overlapping vectors per lane for each it quantises 25, 88 and 59 us.
 template <typename T, int CPL, int WPR>
-__global__ void __launch_bounds__(kThreads, 4) quantizeRowsOddKernel(int64_t const rows, int32_t const width, T const* __restrict__ in,
+__global__ void __launch_bounds__(kThreads, 4) quantizeRowsOddKernel(int64_t const rows, int32_t const width, T const* in,
     int64_t const inStride, int8_t* __restrict__ out, int64_t const outStride, float* __restrict__ scales)
 {
     constexpr int E = Chunk<T>::kElems;
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 4) quantizeRowsOddKernel(int64_t con
 // Rows longer than the registers of eight warps, or whose results are not aligned for wide stores: a CTA per row reads it twice (the second time from
 // L1 or L2), one value per lane.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) quantizeRowsLongKernel(int64_t const rows, int32_t const width, T const* __restrict__ in,
+__global__ void __launch_bounds__(kThreads) quantizeRowsLongKernel(int64_t const rows, int32_t const width, T const* in,
     int64_t const inStride, int8_t* __restrict__ out, int64_t const outStride, float* __restrict__ scales)
 {
     __shared__ float red[2][kThreads / 32];
@@ -326,9 +326,17 @@ __global__ void __launch_bounds__(kThreads) quantizeRowsLongKernel(int64_t const
         RowScale const s = makeRowScale(m);
         if (threadIdx.x == 0)
             scales[row] = rowScaleValue(m);
-#pragma unroll 8
-        for (int i = threadIdx.x; i < width; i += kThreads)
-            out[row * outStride + i] = quantRowValue<sizeof(T) == 4>(static_cast<float>(p[i]), s);
+        for (int i0 = threadIdx.x; i0 < width; i0 += 8 * kThreads)
+        {
+            float v[8]; // all of them on their way before the first result is stored
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[j] = i0 + j * kThreads < width ? static_cast<float>(p[i0 + j * kThreads]) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i0 + j * kThreads < width)
+                    out[row * outStride + i0 + j * kThreads] = quantRowValue<sizeof(T) == 4>(v[j], s);
+        }
     }
 }
 

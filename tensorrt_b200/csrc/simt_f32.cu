@@ -304,11 +304,11 @@ __device__ __forceinline__ SeqRows seqRows(int b, int B, int S, int32_t const* c
 // Four consecutive elements of a row, as FP32.
 __device__ __forceinline__ float4 load4(float const* p)
 {
-    return __ldg(reinterpret_cast<float4 const*>(p));
+    return ldGlobal(reinterpret_cast<float4 const*>(p));
 }
 __device__ __forceinline__ float4 load4(__half const* p)
 {
-    uint2 const v = __ldg(reinterpret_cast<uint2 const*>(p));
+    uint2 const v = ldGlobal(reinterpret_cast<uint2 const*>(p));
     float2 const lo = __half22float2(*reinterpret_cast<__half2 const*>(&v.x));
     float2 const hi = __half22float2(*reinterpret_cast<__half2 const*>(&v.y));
     return make_float4(lo.x, lo.y, hi.x, hi.y);
@@ -390,7 +390,7 @@ __device__ __forceinline__ void addFourKeys(Smem const& sm, int const row0, int 
 // SKIP: keys beyond the sequence, which have no weight, are left out of the second product, four or eight at a time (the scores' product takes all 64).
 template <typename T, int D, int WARPS, bool ASYNC, bool SKIP>
 __global__ void __launch_bounds__(32 * WARPS) mhaTiledKernel(int32_t const B, int32_t const S, int32_t const N, int32_t const d,
-    T const* __restrict__ qkv, T* __restrict__ out, int32_t const* __restrict__ cu, int32_t const* __restrict__ maskIdx, float const scale)
+    T const* qkv, T* __restrict__ out, int32_t const* cu, int32_t const* maskIdx, float const scale)
 {
     static_assert(!ASYNC || (sizeof(T) == 4 && SKIP), "FP16 is converted on the way");
     extern __shared__ float smRaw[];

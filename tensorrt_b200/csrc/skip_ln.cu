@@ -125,9 +125,12 @@ __device__ __forceinline__ void prefetchParams(int32_t ld, T const* beta, T cons
 // One row is shared by WPR warps; each lane owns CPL 16-byte chunks: chunk (i*WPR + wInRow)*32 + lane.
 // The grid strides over rows, so gamma/beta/bias chunks (always the same columns for a lane) stay
 // in L1 after the first row.
-template <typename T, int CPL, int WPR, bool HAS_BIAS>
-__global__ void __launch_bounds__(kThreads, (WPR == 2 && CPL == 2) ? 4 : 1) skipLnKernel(int32_t const ld, int64_t const rows, T const* __restrict__ in,
-    T const* __restrict__ skip, T const* __restrict__ beta, T const* __restrict__ gamma, T const* __restrict__ bias,
+// EARLY (CTAs that have an SM each, so that latency counts and registers don't): a row's gamma and beta are on their way before its variance is known. Otherwise each
+// chunk's are loaded when it is stored, behind the store of the chunk before: 37 x 1024 FP32 2.5 / 1.9 us, FP16 x 768 2.3 / 1.8 us, x 4096 2.7 / 2.1 us, but
+// 6000 x 4096 FP32 48.7 / 59.9 us, FP16 27.4 / 37.3 us, 24576 x 768 19.5 / 21.9 us.
+template <typename T, int CPL, int WPR, bool HAS_BIAS, bool EARLY>
+__global__ void __launch_bounds__(kThreads, (WPR == 2 && CPL == 2) ? 4 : 1) skipLnKernel(int32_t const ld, int64_t const rows, T const* in,
+    T const* skip, T const* beta, T const* gamma, T const* bias,
     T* __restrict__ out, float const eps)
 {
     constexpr int E = Vec<T>::kElems;
@@ -215,6 +218,20 @@ __global__ void __launch_bounds__(kThreads, (WPR == 2 && CPL == 2) ? 4 : 1) skip
                 }
             }
         }
+        uint4 early[2][CPL];
+        if (EARLY)
+        {
+#pragma unroll
+            for (int i = 0; i < CPL; ++i)
+            {
+                int const c = (i * WPR + wInRow) * 32 + lane;
+                if (c < chunksPerRow)
+                {
+                    early[0][i] = ldgKeep(gamma + c * E);
+                    early[1][i] = ldgKeep(beta + c * E);
+                }
+            }
+        }
         float const var = rowSum<WPR>(q, red[rowInCta], rowInCta, wInRow, lane, turn) * rld;
         float const rsigma = rsqrtf(var + eps);
 
@@ -225,8 +242,8 @@ __global__ void __launch_bounds__(kThreads, (WPR == 2 && CPL == 2) ? 4 : 1) skip
             if (rowOk && c < chunksPerRow)
             {
                 float g[E], bt[E];
-                Vec<T>::unpack(ldgKeep(gamma + c * E), g);
-                Vec<T>::unpack(ldgKeep(beta + c * E), bt);
+                Vec<T>::unpack(EARLY ? early[0][i] : ldgKeep(gamma + c * E), g);
+                Vec<T>::unpack(EARLY ? early[1][i] : ldgKeep(beta + c * E), bt);
 #pragma unroll
                 for (int j = 0; j < E; ++j)
                     x[i][j] = g[j] * (x[i][j] - mu) * rsigma + bt[j];
@@ -274,8 +291,8 @@ __global__ void __launch_bounds__(kThreads) skipLnScalarKernel(int32_t const ld,
 // INT8 linear rows: 16 values per 128-bit load, FP16 parameters (two 128-bit loads per chunk).
 template <int CPL, int WPR, bool HAS_BIAS>
 __global__ void __launch_bounds__(kThreads) skipLnDqqKernel(int32_t const ld, int64_t const rows,
-    int8_t const* __restrict__ in, int8_t const* __restrict__ skip, __half const* __restrict__ beta,
-    __half const* __restrict__ gamma, __half const* __restrict__ bias, int8_t* __restrict__ out, float const dqIn,
+    int8_t const* in, int8_t const* skip, __half const* beta,
+    __half const* gamma, __half const* bias, int8_t* __restrict__ out, float const dqIn,
     float const dqSkip, float const qScale, float const eps)
 {
     constexpr int E = 16;
@@ -403,8 +420,8 @@ __global__ void __launch_bounds__(kThreads) skipLnDqqKernel(int32_t const ld, in
 // exactly three chunks of 8 per lane).
 template <int CPL, int WPR, bool HAS_BIAS, int CB = 16>
 __global__ void __launch_bounds__(kThreads, 3) skipLnDqqPackedKernel(int32_t const ld, int64_t const rows,
-    int8_t const* __restrict__ in, int8_t const* __restrict__ skip, __half const* __restrict__ beta,
-    __half const* __restrict__ gamma, __half const* __restrict__ bias, int8_t* __restrict__ out, float const dqIn,
+    int8_t const* in, int8_t const* skip, __half const* beta,
+    __half const* gamma, __half const* bias, int8_t* __restrict__ out, float const dqIn,
     float const dqSkip, float const qScale, float const eps, bool const paramsReady)
 {
     constexpr int E = CB;
@@ -961,12 +978,10 @@ int32_t launchSkipLn(cudaStream_t stream, int32_t ld, int64_t rows, T const* in,
 {
     int const rowsPerCta = kWarpsPerCta / WPR;
     int const grid = gridFor((rows + rowsPerCta - 1) / rowsPerCta, 8);
-    if (bias)
-        launchDependent(skipLnKernel<T, CPL, WPR, true>, dim3(grid), dim3(kThreads), 0, stream, ld, rows, in, skip, beta, gamma, bias,
-            out, eps);
-    else
-        launchDependent(skipLnKernel<T, CPL, WPR, false>, dim3(grid), dim3(kThreads), 0, stream, ld, rows, in, skip, beta, gamma, bias,
-            out, eps);
+    bool const early = grid <= smCount() && !(CPL == 2 && WPR == 2); // (kept to 64 registers: 37 x 1024 FP16 2.2 / 2.3 us)
+    auto const kernel = bias ? (early ? skipLnKernel<T, CPL, WPR, true, true> : skipLnKernel<T, CPL, WPR, true, false>)
+                             : (early ? skipLnKernel<T, CPL, WPR, false, true> : skipLnKernel<T, CPL, WPR, false, false>);
+    launchDependent(kernel, dim3(grid), dim3(kThreads), 0, stream, ld, rows, in, skip, beta, gamma, bias, out, eps);
     return checkLaunch("skipLnKernel");
 }
 

@@ -75,8 +75,8 @@ constexpr int kCtasPerSm = CPL == 1 ? 3 : 2;
 // largest magnitude. Arithmetic for pairs of values: with one value per instruction (36 of them each) the kernel was bound by issue slots.
 template <typename T, int CPL, int WPR, bool HAS_BIAS>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm<CPL>) skipLnQuantKernel(int32_t const ld, int64_t const rows,
-    T const* __restrict__ in, T const* __restrict__ skip, T const* __restrict__ beta, T const* __restrict__ gamma, T const* __restrict__ bias,
-    T* __restrict__ out, float const eps, int8_t* __restrict__ outI8, float* __restrict__ rowScales)
+    T const* in, T const* skip, T const* beta, T const* gamma, T const* bias,
+    T* out, float const eps, int8_t* __restrict__ outI8, float* __restrict__ rowScales)
 {
     constexpr int E = Pairs<T>::kElems;
     constexpr int P = E / 2;
@@ -269,7 +269,7 @@ __host__ __device__ constexpr int oddRowBytes(int slots) // of a row in shared m
 
 template <typename T, int NV, int WPR, bool HAS_BIAS>
 __global__ void __launch_bounds__(kThreads, NV <= 8 ? 4 : NV <= 16 ? 3 : 2) skipLnQuantOddKernel(int32_t const ld, int64_t const rows, T const* in, T const* skip,
-    T const* __restrict__ beta, T const* __restrict__ gamma, T const* __restrict__ bias, T* out, float const eps, int8_t* __restrict__ outI8,
+    T const* beta, T const* gamma, T const* bias, T* out, float const eps, int8_t* __restrict__ outI8,
     float* __restrict__ rowScales)
 {
     constexpr int kRowsPerCta = kWarpsPerCta / WPR;
