@@ -130,8 +130,9 @@ class PoolerHead:
 class MaskedLmHead:
     """The head of `BertForMaskedLM` (`cls.predictions`: dense + erf-GELU + LayerNorm, then the product with the vocabulary) on top of the
     encoder output, and what it is asked: log probabilities of given tokens, entropy, the most likely tokens. The product with the vocabulary is
-    usually tied to the word embeddings (no `decoder.weight` in the state dict). rowwise=True: both products in INT8 with a scale per token and per
-    output channel, logits FP32; False: FP16."""
+    usually tied to the word embeddings (no `decoder.weight` in the state dict). rowwise=True, which is what a caller gets who chooses nothing, also on
+    an FP16 encoder: both products in INT8 with a scale per token and per output channel, logits FP32. False: both products in FP16, logits FP16, so that
+    log probabilities carry the logits' rounding (2^-11 of their size: 1e-2 at logits of 20)."""
 
     def __init__(self, state_dict, device="cuda:0", rowwise=True, eps=1e-12):
         import torch
@@ -182,7 +183,8 @@ class MaskedLmHead:
         return ops.fc(y, self.decoder, self.bias)[:, :self.vocab]
 
     def __call__(self, hidden, positions=None, token_ids=None, top_k=5):
-        """hidden: FP16 [total, hidden] (packed tokens); positions: the rows that are asked about (None: all); token_ids: int32 [positions, tokens] or
+        """hidden: FP16 [total, hidden] (packed tokens); positions: the rows that are asked about (None: all), each within
+        [0, total) (they are not looked at on the host); token_ids: int32 [positions, tokens] or
         [positions] -> ops.LogProbs."""
         from . import ops
 

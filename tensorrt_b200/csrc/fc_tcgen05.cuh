@@ -65,8 +65,9 @@ inline FcProblem plainFc(bert_b200_fc_params const& p)
 // erf-GELU through a fitted tanh form: gelu(x) = x/2 * (1 + tanh(x * (c1 + c3 x^2 + c5 x^4))), x^2 clamped at 64.
 // The three coefficients are a minimax fit against 0.5 x (1 + erf(x / sqrt 2)) on [-9, 9]: |error| <= 2.6e-5
 // (the classic 0.044715 cubic form is off by 4.7e-4). On top comes the error of the hardware tanh.approx
-// (about 2^-11 relative), i.e. at most ~2.5e-4 |x| absolute - below FP16 resolution of the result and about
-// 1 % of an INT8 step. Cost: 5 FMA-pipe operations and one MUFU operation per value.
+// (about 2^-11 relative), i.e. at most ~2.5e-4 |x| absolute - below half an FP16 step of the result for large x, about
+// 1 % of an INT8 step, but more than the small results of the negative tail are precise to in FP16 (measured there: 4.3e-5 at
+// x = -2 ... -3, 2.7e-5 below). Cost: 5 FMA-pipe operations and one MUFU operation per value.
 constexpr float kGeluC1 = 7.97507884e-01f;
 constexpr float kGeluC3 = 3.70056460e-02f;
 constexpr float kGeluC5 = -3.51516788e-04f;

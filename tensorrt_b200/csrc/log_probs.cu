@@ -15,10 +15,15 @@
 // Few rows may be shared by a cluster of CTAs each: their last warps hand what they found to the first CTA's through distributed shared memory. Such
 // a cluster has one row only (clusterFor), so no place there is used twice.
 //
-// Bound by issue slots: of some 10000 warp instructions of a row of 30522 halves, 4000 are exponentials (34 per eight values: conversion, one
-// multiply-add, ex2, two sums, clamp), 700 the maximum, 900 copies, the rest per row and warp; 0.60 of the slots are used with 27 warps per SM. 3686 x
-// 30522 FP16, top 10: 54.7 us, 4.1 TB/s (floor 34.9 us; 146 us with rows in registers, 102 us with everything in turn); FP32 888 rows without
-// likely tokens 21.6 us, 5.0 TB/s. One row 5.7 us.
+// Of some 10000 warp instructions of a row of 30522 halves, 4000 are exponentials (34 per eight values: conversion, one multiply-add, ex2, two sums,
+// clamp), 700 the maximum, 900 copies, the rest per row and warp. 0.63 of the issue slots are used with 24 warps per SM; a warp's other cycles go to
+// dependent instructions, the CTA's barriers and shared memory. 3686 x 30522 FP16, top 10: 55.4 us, 4.1 TB/s (floor 34.9 us; 146 us with rows in registers, 102 us with
+// everything in turn); FP32 888 rows without likely tokens 23.7 us, 4.6 TB/s. One row 5.7 us. Short rows: 0.64 of the slots (20000 x 2000 FP16, top 10, 51 us, floor
+// 12.5 us), every step of a row behind the one before it in the same warp.
+// Slow, though right: parts whose list overflows. Those are parts with fewer than topK values above one that hundreds share (masks of the type's lowest value,
+// equal logits: 30522 values, top 5, one FP16 row with three tokens left 47 us instead of 6, 400 FP32 rows whose second half, a part, is masked 53 us instead of 14, 3686
+// FP16 rows of equal values 530 us instead of 53; without likely tokens such values are only counted: 31 us instead of 13 for those 400 rows), and, for 17 to 20 tokens,
+// up to 444 rows of 65 to 76 vectors, which leave some of the 32 pairs of groups empty (FP16 505 ... 608, FP32 256 ... 304 values: 12 ... 33 us instead of 4 ... 7).
 #include "sm100.cuh"
 
 namespace b200

@@ -175,8 +175,8 @@ __global__ void __launch_bounds__(kThreads) quantizeRowsKernel(int64_t const row
 }
 
 // Rows that begin at any value: the 16-byte vectors that hold them are quantised as they lie, `mis` values behind the row's; what moves by `mis` is
-// the results, a quarter or half as many bytes: a lane's vector and its neighbour's, together, hold the bytes it stores. Bound by issue slots (110
-// instructions per vector and warp). FP16 24576 x 1001 19.3 us (17.5 us on 16 bytes), x 4095 79 us (52), FP32 12000 x 4097 49 us (39); with one value per
+// the results, a quarter or half as many bytes: a lane's vector and its neighbour's, together, hold the bytes it stores. Mostly issue slots (110
+// instructions per vector and warp; 72 % of the slots used at 24576 x 4095 FP16, the rest waits for the row's loads and its maximum). FP16 24576 x 1001 19.3 us (17.5 us on 16 bytes), x 4095 79 us (52), FP32 12000 x 4097 49 us (39); with one value per
 // lane and load 61, 115 and 59 us, with two overlapping vectors per lane for each it quantises 25, 88 and 59 us.
 template <typename T, int CPL, int WPR>
 __global__ void __launch_bounds__(kThreads, 4) quantizeRowsOddKernel(int64_t const rows, int32_t const width, T const* in,
@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(kThreads, 4) quantizeRowsOddKernel(int64_t con
 }
 
 // Rows longer than the registers of eight warps, or whose results are not aligned for wide stores: a CTA per row reads it twice (the second time from
-// L1 or L2), one value per lane.
+// L1 or L2), one value per lane and load. FP32 6000 x 8192 64 us (floor 38 us), FP16 3000 x 14336 54 us (20 us), 3000 x 8200
+// 32.2 us (11.4 us): the loads of single values, not the memory.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantizeRowsLongKernel(int64_t const rows, int32_t const width, T const* in,
     int64_t const inStride, int8_t* __restrict__ out, int64_t const outStride, float* __restrict__ scales)

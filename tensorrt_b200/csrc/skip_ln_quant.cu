@@ -253,8 +253,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<CPL>) skipLnQuantKernel(i
 // Rows that cannot be read 16 bytes at a time: WPR warps per row, each with NV neighbouring values per lane, 32 apart, in registers, so that the sums
 // can be those of one warp that goes along the row (skip_ln.cu's scalar kernel, to the bit): each warp goes on where the one before it ended.
 // The next row's 16-byte vectors are on their way to shared memory meanwhile, where single values are read from; the parameters are
-// there for the whole launch. Bound by issue slots (some 35 instructions per value). FP16 24576 x 1001 44.8 us (x 1024 34.5 us; 116 us with the kernel below),
-// FP32 12000 x 1001 33.9 us (81 us), FP16 3000 x 4001 43 us (74 us), 37 x 1001 4.5 us (11.4 us).
+// there for the whole launch. Some 35 instructions per value; up to 1024 values (a warp per row) issue slots bound it, beyond that the order of the sums:
+// the row's warps add one after the other, twice, and most of them wait (3000 x 4001 FP16: 42 % of the slots used, 13 warps per SM; of a warp's 8 cycles
+// per instruction 2.0 for loads, 1.5 at barriers). FP16 24576 x 1001 44.8 us (x 1024 34.0 us; 116 us with the kernel below), FP32 12000 x 1001 33.9 us (81 us), FP16
+// 3000 x 4001 43 us (74 us), 2957 x 2543 32.7 us, 37 x 1001 4.5 us (11.4 us). Aligned FP32 rows of 4100 to 8192 values come here too, since skip_layer_norm sums
+// them in this order, one CTA per SM by their shared memory: 1500 x 4100 56 us, 1500 x 8192 64 us (floor 24.7 us; skip_layer_norm 297 us).
 template <typename T>
 struct alignas(2 * sizeof(T)) GammaBeta
 {
@@ -435,7 +438,8 @@ __global__ void __launch_bounds__(kThreads, NV <= 8 ? 4 : NV <= 16 ? 3 : 2) skip
     }
 }
 
-// Longer rows, scalar accesses, one warp per row; the row is revisited from L1 / L2 instead of registers.
+// Longer rows, scalar accesses, one warp per row; the row is revisited from L1 / L2 instead of registers. 1500 x 12288 FP16 274 us, FP32 391 us (skip_layer_norm,
+// in the same order, 228 us FP16).
 template <typename T, bool HAS_BIAS>
 __global__ void __launch_bounds__(kThreads) skipLnQuantScalarKernel(int32_t const ld, int64_t const rows, T const* in, T const* skip,
     T const* __restrict__ beta, T const* __restrict__ gamma, T const* __restrict__ bias, T* out, float const eps, int8_t* __restrict__ outI8,

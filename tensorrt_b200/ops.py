@@ -275,7 +275,8 @@ class LogProbs(NamedTuple):
 def token_log_probs(logits, token_ids=None, top_k=0, status=None):
     """Log probabilities of given tokens, entropy and the top_k (at most 32) most likely tokens of each row of FP16/FP32 logits [rows, vocab], a
     matrix or a view with a row stride. token_ids: int32 [rows, tokens] or [rows]; ids outside the vocabulary have probability 0. Tokens of
-    logit -inf are no alternatives (ids -1 where too few are left); rows with NaN or +inf give NaN."""
+    logit -inf are no alternatives (ids -1 where too few are left); rows with NaN or +inf give NaN. Masks of the type's lowest value are
+    right but slow where they leave less than top_k tokens of a long stretch of the vocabulary (it is read twice): mask with -inf."""
     _here(logits, token_ids, status)
     if (logits.dtype is not torch.float16 and logits.dtype is not torch.float32) or logits.dim() != 2:
         raise ValueError(f"token_log_probs takes float16 or float32 logits [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
