@@ -261,7 +261,7 @@ BERT_B200_API int32_t bert_b200_quantize_rows(void* stream, int32_t type_id, int
  * each output channel, INT32 sums (exact; k <= 131071), C FP16 or FP32 (out_type_id 1 or 0), bias FP32 or NULL, act per `activation`.
  * Any m, n and k; lda, ldw, ldc are row strides in elements, each a multiple of 16 bytes; A, Wt and C 16-byte aligned.
  * Only the m x n values of C are written. A row of C has the same bits whatever m. With FP16 results the GELU is the fitted form of
- * bert_b200_fc, off by at most 2.6e-5 + |x| 2^-12 beside the result's rounding: an absolute bound, so that results near 0 in the negative tail keep
+ * bert_b200_fc, off by at most 2.6e-5 + |x| (2^-12 + 2^-20) beside the result's rounding: an absolute bound, so that results near 0 in the negative tail keep
  * no relative precision (measured there: 4.3e-5 at x = -2 ... -3, 2.7e-5 below). With FP32 results it is taken with erff. `status_word` as in bert_b200_fc.
  * ref: none (plugin/fcPlugin/fcPlugin.cpp:551-610 has no INT8 scales)
  */

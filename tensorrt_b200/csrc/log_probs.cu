@@ -17,7 +17,7 @@
 //
 // Of some 10000 warp instructions of a row of 30522 halves, 4000 are exponentials (34 per eight values: conversion, one multiply-add, ex2, two sums,
 // clamp), 700 the maximum, 900 copies, the rest per row and warp. 0.63 of the issue slots are used with 24 warps per SM; a warp's other cycles go to
-// dependent instructions, the CTA's barriers and shared memory. 3686 x 30522 FP16, top 10: 55.4 us, 4.1 TB/s (floor 34.9 us; 146 us with rows in registers, 102 us with
+// dependent instructions, the CTA's barriers and shared memory. 3686 x 30522 FP16, top 10: 54.9 us, 4.1 TB/s (floor 34.9 us; 146 us with rows in registers, 102 us with
 // everything in turn); FP32 888 rows without likely tokens 23.7 us, 4.6 TB/s. One row 5.7 us. Short rows: 0.64 of the slots (20000 x 2000 FP16, top 10, 51 us, floor
 // 12.5 us), every step of a row behind the one before it in the same warp.
 // Slow, though right: parts whose list overflows. Those are parts with fewer than topK values above one that hundreds share (masks of the type's lowest value,
@@ -712,26 +712,29 @@ __device__ __forceinline__ void writeRow(LogProbsArgs const& args, Result const&
     };
     if (lane < args.numTokens)
         args.logProbs[r * args.numTokens + lane] = logProb(tokenLogit);
-    // Many tokens: eight of a lane at a time, the next eight on their way with these ones' logits.
-    constexpr int kAtOnce = 8;
-    auto loadTokens = [&](int j0, int32_t (&token)[kAtOnce]) {
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            token[i] = j0 + 32 * i < args.numTokens ? ldGlobal(args.tokenIds + r * args.numTokens + j0 + 32 * i) : -1;
-    };
-    int32_t token[kAtOnce];
-    loadTokens(lane + 32, token);
-    for (int j0 = lane + 32; j0 < args.numTokens; j0 += kAtOnce * 32)
+    if (args.numTokens > 32)
     {
-        float x[kAtOnce];
+        // four of a lane at a time, the next four on their way with these ones' logits: 30522 tokens of a row 74 us, one by one 350 us
+        constexpr int kAtOnce = 4;
+        auto loadTokens = [&](int j0, int32_t (&token)[kAtOnce]) {
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            x[i] = token[i] >= 0 && token[i] < args.vocab ? static_cast<float>(ldGlobal(row.p + token[i])) : negInf();
-        loadTokens(j0 + kAtOnce * 32, token);
+            for (int i = 0; i < kAtOnce; ++i)
+                token[i] = j0 + 32 * i < args.numTokens ? ldGlobal(args.tokenIds + r * args.numTokens + j0 + 32 * i) : -1;
+        };
+        int32_t token[kAtOnce];
+        loadTokens(lane + 32, token);
+        for (int j0 = lane + 32; j0 < args.numTokens; j0 += kAtOnce * 32)
+        {
+            float x[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            if (j0 + 32 * i < args.numTokens)
-                args.logProbs[r * args.numTokens + j0 + 32 * i] = logProb(x[i]);
+            for (int i = 0; i < kAtOnce; ++i)
+                x[i] = token[i] >= 0 && token[i] < args.vocab ? static_cast<float>(ldGlobal(row.p + token[i])) : negInf();
+            loadTokens(j0 + kAtOnce * 32, token);
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                if (j0 + 32 * i < args.numTokens)
+                    args.logProbs[r * args.numTokens + j0 + 32 * i] = logProb(x[i]);
+        }
     }
     if (lane == 0 && args.entropy)
         args.entropy[r] = bad ? nan : none ? 0.f : lse - st.t / (st.count + st.s);
